@@ -21,6 +21,7 @@ sources = [
     os.path.join(CSRC, "elementwise.hip"),
     os.path.join(CSRC, "loss.hip"),
     os.path.join(CSRC, "step.hip"),
+    os.path.join(CSRC, "adamw.hip"),
     os.path.join(CSRC, "aug_kernels.hip"),
     os.path.join(CSRC, "bnrelu.hip"),
     os.path.join(CSRC, "conv_mfma.hip"),
@@ -35,7 +36,9 @@ setup(
             sources=sources,
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],
-                "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+                # no packed-fp32 instructions: some forms of them are not reliable
+                "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
             },
         )
     ],
