@@ -23,6 +23,11 @@ void rmsprop_fused_step_mixed(torch::Tensor master, torch::Tensor work, torch::T
                               torch::Tensor ms, torch::Tensor mom, torch::Tensor normsq,
                               torch::Tensor lr_t, int64_t n_decay, double wd,
                               double clip, double rho, double momentum, double eps);
+void adamw_step(std::vector<torch::Tensor> rows, std::vector<torch::Tensor> chunks,
+                std::vector<int64_t> kinds, torch::Tensor m, torch::Tensor r,
+                torch::Tensor m_scale, torch::Tensor r_scale, torch::Tensor step,
+                torch::Tensor scal, torch::Tensor part, torch::Tensor lr, double b1,
+                double b2, double eps, double clip);
 torch::Tensor aug_pipeline(torch::Tensor images, torch::Tensor sel, torch::Tensor prog,
                            torch::Tensor post, torch::Tensor mean, torch::Tensor std,
                            bool bf16_out);
@@ -79,6 +84,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ema_lerp_", &ema_lerp_);
   m.def("rmsprop_fused_step_mixed", &rmsprop_fused_step_mixed,
         "fused TF-semantics RMSprop on flat mixed-precision buffers");
+  m.def("adamw_step", &adamw_step,
+        "AdamW over a table of tensors, moments in fp32 or in e4m3 blocks");
   m.def("gather_grads", &gather_grads,
         "pack scattered autograd grads into the flat bf16 buffer");
   m.def("aug_pipeline_imagenet", &aug_pipeline_imagenet,

@@ -13,8 +13,15 @@ parallel.flat), and one step = three HIP kernels over contiguous memory:
   2. l2norm:    ||g||^2 of the whole flat grad -> 1-elem device tensor
   3. sgd_step:  clip coef read on-device, nesterov momentum update
 No host sync anywhere, so the whole step is hipGraph-capturable.
+
+FusedAdamW is AdamW (decoupled decay) over the same flat buffers or over any
+list of tensors, with its two moments in 32 or in 8 bits: one launch for all
+tensors, one more for the step's scalars and one for the norm if it clips.
 """
 from __future__ import annotations
+
+import math
+import struct
 
 import torch
 from torch.optim.optimizer import Optimizer
@@ -237,3 +244,299 @@ class FusedRMSpropTF:
     def load_state_dict(self, sd):
         self.ms.copy_(sd["ms"])
         self.mom.copy_(sd["mom"])
+
+
+class FusedAdamW:
+    """AdamW over all tensors of a model at once, moments in 32 or 8 bits.
+
+        g' = g * min(1, grad_clip / (||g|| + 1e-6))      (grad_clip > 0; norm over all tensors)
+        m  = b1 m + (1-b1) g'        v = b2 v + (1-b2) g'^2
+        p  = p (1 - lr wd) - lr (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
+
+    ``params`` is a ``parallel.flat.FlatParams`` (its decay segment decays, the
+    rest does not), an iterable of parameters, or a list of
+    ``{"params": [...], "weight_decay": w}`` groups. Parameters are contiguous,
+    fp32, bf16 or fp16, and all on one device; bf16 and fp16 ones get fp32
+    weights that the optimizer keeps (FlatParams brings its own), which are
+    updated and rounded back into the parameters. A parameter whose ``grad`` is
+    None is left as it is. The step count is one for all parameters.
+
+    ``state_bits=8`` holds m and sqrt(v) as e4m3 numbers (``exp_avg``,
+    ``exp_avg_root``) with one fp32 scale for every 256 neighbours of a tensor
+    (``*_scale``); the step uses the moments before they are rounded. A flat
+    buffer then has to start each tensor at a multiple of 256
+    (``flatten_module(align=256)``). A block with a NaN or an infinity in it is
+    no number as a whole from then on.
+
+    The step count and the learning rate are on the device: a captured step
+    replays, with ``sync_lr()`` before a replay pushing a changed rate. Under
+    capture the gradients have to be where an eager step saw them.
+    """
+
+    BLOCK = 256         # elements under one scale
+    CHUNK = 4096        # elements a workgroup takes
+    _NORM_PARTS = 1024
+    _KINDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.0, grad_clip: float = 0.0, state_bits: int = 32):
+        b1, b2 = (float(b) for b in betas)
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"FusedAdamW: betas={betas} have to lie in [0, 1)")
+        if not (eps > 0.0 and lr >= 0.0 and weight_decay >= 0.0 and grad_clip >= 0.0):
+            raise ValueError("FusedAdamW: eps > 0 and lr, weight_decay, grad_clip >= 0 are needed")
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdamW: state_bits={state_bits} is neither 8 nor 32")
+        self.betas, self.eps = (b1, b2), float(eps)
+        self.weight_decay, self.grad_clip, self.state_bits = float(weight_decay), float(grad_clip), state_bits
+        self.flat = params if hasattr(params, "flat_param") else None
+        if self.flat is not None:
+            total = self._init_flat()
+        else:
+            total = self._init_list(params)
+        self.lr = lr
+        self.param_groups = [{"lr": lr}]
+        self._last_lr = lr
+        dev = self._dev
+        zeros = lambda n, t: torch.zeros(n, dtype=t, device=dev)  # noqa: E731
+        if state_bits == 32:
+            self.exp_avg, self.exp_avg_sq = zeros(total, torch.float32), zeros(total, torch.float32)
+            self._names = ("exp_avg", "exp_avg_sq")
+        else:
+            total = -(-total // self.BLOCK) * self.BLOCK
+            self.exp_avg, self.exp_avg_root = (
+                zeros(total, torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+            self.exp_avg_scale = zeros(total // self.BLOCK, torch.float32)
+            self.exp_avg_root_scale = zeros(total // self.BLOCK, torch.float32)
+            self._names = ("exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale")
+        self.step_count = zeros(1, torch.int64)
+        self._lr_t = torch.full((1,), lr, device=dev, dtype=torch.float32)
+        self._scal = zeros(3, torch.float32)
+        self._part = zeros(self._NORM_PARTS * 3, torch.float32)
+        self._seen = None       # addresses that the tables on the device were made for
+        self._tables = None
+
+    # ---- what there is to update: (weights fp32, low-precision copy, gradient's owner, offset, n, decay)
+
+    def _init_flat(self):
+        f = self.flat
+        n, nd = f.flat_param.numel(), f.n_decay
+        if f.flat_param.dtype not in self._KINDS or f.flat_grad.dtype != f.flat_param.dtype:
+            raise TypeError("FusedAdamW: flat buffers are fp32, bf16 or fp16, weights and gradients alike")
+        if f.flat_param.dtype != torch.float32 and f.flat_master is None:
+            raise ValueError("FusedAdamW: low-precision flat weights need flat_master")
+        if self.state_bits == 8 and (nd % self.BLOCK or any(
+                (p.data_ptr() - f.flat_param.data_ptr()) // f.flat_param.element_size() % self.BLOCK
+                for p in f.params)):
+            raise ValueError("FusedAdamW: 8-bit moments need tensors that start at multiples of "
+                             "256 in the flat buffer: flatten_module(align=256)")
+        self._dev = f.flat_param.device
+        self._items = [(0, nd, self.weight_decay), (nd, n - nd, 0.0)]
+        return n
+
+    def _init_list(self, params):
+        groups = list(params)
+        if not groups:
+            raise ValueError("FusedAdamW: no parameters")
+        if not isinstance(groups[0], dict):
+            groups = [{"params": groups}]
+        self.params, self._items, total, seen = [], [], 0, set()
+        for g in groups:
+            odd = set(g) - {"params", "weight_decay"}
+            if odd:
+                raise ValueError(f"FusedAdamW: a group holds params and weight_decay, not {sorted(odd)}")
+            wd = float(g.get("weight_decay", self.weight_decay))
+            if not wd >= 0.0:
+                raise ValueError("FusedAdamW: weight_decay >= 0 is needed")
+            ps = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            for p in ps:
+                if p.dtype not in self._KINDS:
+                    raise TypeError(f"FusedAdamW: a parameter of {p.dtype}: fp32, bf16 and fp16 are stepped")
+                if id(p) in seen:
+                    raise ValueError("FusedAdamW: a parameter is listed twice")
+                seen.add(id(p))
+                self.params.append(p)
+                self._items.append((total, p.numel(), wd))
+                total += -(-p.numel() // self.BLOCK) * self.BLOCK
+        if not self.params:
+            raise ValueError("FusedAdamW: no parameters")
+        self._dev = self.params[0].device
+        if any(p.device != self._dev for p in self.params):
+            raise ValueError("FusedAdamW: the parameters are on several devices")
+        self.masters = [None if p.dtype == torch.float32 else p.detach().float() for p in self.params]
+        return total
+
+    @staticmethod
+    def _same_order(a, b):
+        """Whether two tensors of one shape lie in memory in the same order, without gaps."""
+        return (a.is_contiguous() and b.is_contiguous()) or (
+            a.stride() == b.stride() and a.dim() == 4 and a.is_contiguous(memory_format=torch.channels_last))
+
+    def _views(self):
+        """(type, fp32 weights, low-precision copy or None, gradient or None, offset, n, decay) of every tensor."""
+        if self.flat is not None:
+            f = self.flat
+            low = f.flat_param if f.flat_param.dtype != torch.float32 else None
+            full = f.flat_param if low is None else f.flat_master
+            return [(f.flat_param.dtype, full[off:off + n], None if low is None else low[off:off + n],
+                     f.flat_grad[off:off + n], off, n, wd) for off, n, wd in self._items if n > 0]
+        views = []
+        for p, master, (off, n, wd) in zip(self.params, self.masters, self._items):
+            if n == 0:
+                continue
+            w, low = (p.detach(), None) if master is None else (master, p.detach())
+            if p.numel() != n or p.device != self._dev or not self._same_order(p, w):
+                raise ValueError("FusedAdamW: a parameter is not contiguous, or changed its size, device or order")
+            g = p.grad
+            if g is not None:
+                if g.layout != torch.strided or g.dtype != p.dtype or g.device != self._dev or g.shape != p.shape:
+                    raise TypeError("FusedAdamW: a gradient is sparse, or of another type, shape or device than its parameter")
+                if not self._same_order(g, p):
+                    p.grad = g = torch.empty_like(p).copy_(g)
+            views.append((p.dtype, w, low, g, off, n, wd))
+        return views
+
+    def _addresses(self):
+        """What the device tables depend on: every tensor's place and memory order."""
+        if self.flat is not None:
+            f = self.flat
+            return (f.flat_param.data_ptr(), f.flat_grad.data_ptr(),
+                    0 if f.flat_master is None else f.flat_master.data_ptr())
+        return [(p.data_ptr(), p.stride()) if p.grad is None else
+                (p.data_ptr(), p.stride(), p.grad.data_ptr(), p.grad.stride()) for p in self.params]
+
+    def _refresh_tables(self):
+        """The device tables of addresses, made anew where an address changed."""
+        if self._addresses() == self._seen:
+            return self._tables
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: the gradients' addresses changed since the last eager step: "
+                               "keep them in place (zero_grad() fills them) and step once before capture")
+        by = {}
+        for kind, w, low, g, off, n, wd in self._views():
+            rows, chunks = by.setdefault(self._KINDS[kind], ([], []))
+            pw, pl, pg = (0 if t is None else t.data_ptr() for t in (w, low, g))
+            esize = kind.itemsize
+            aligned = pw % 16 == 0 and off % 4 == 0 and pl % (4 * esize) == 0 and pg % (4 * esize) == 0
+            bits = struct.unpack("<I", struct.pack("<f", wd))[0]
+            chunks += [(len(rows), i) for i in range(-(-n // self.CHUNK))]
+            rows.append((pw, pl, pg, off, n, bits | (int(aligned) << 32)))
+        up = lambda v, t, c: torch.tensor(v, dtype=t).view(-1, c).pin_memory().to(self._dev, non_blocking=True)  # noqa: E731
+        if self._tables is not None:    # the old ones may still be read on this stream
+            for t in self._tables[0] + self._tables[1]:
+                t.record_stream(torch.cuda.current_stream(self._dev))
+        self._tables = ([up(r, torch.int64, 6) for r, _ in by.values()],
+                        [up(c, torch.int32, 2) for _, c in by.values()], list(by))
+        self._seen = self._addresses()
+        return self._tables
+
+    def sync_lr(self):
+        """Push param_groups[0]['lr'] to the device scalar (call pre-replay)."""
+        lr = self.param_groups[0]["lr"]
+        if lr != self._last_lr:
+            self._lr_t.fill_(lr)
+            self._last_lr = lr
+
+    def zero_grad(self, set_to_none: bool = False):
+        if self.flat is not None:
+            self.flat.flat_grad.zero_()
+        elif set_to_none:
+            for p in self.params:
+                p.grad = None
+        else:
+            grads = [p.grad for p in self.params if p.grad is not None]
+            if grads:
+                torch._foreach_zero_(grads)
+
+    @torch.no_grad()
+    def step(self):
+        self.lr = self.param_groups[0]["lr"]
+        if self._dev.type != "cuda":
+            return self._step_cpu()
+        from .ops import ext
+        if not torch.cuda.is_current_stream_capturing():
+            self.sync_lr()
+        rows, chunks, kinds = self._refresh_tables()
+        m = self.exp_avg
+        r = self.exp_avg_sq if self.state_bits == 32 else self.exp_avg_root
+        ms = self._scal if self.state_bits == 32 else self.exp_avg_scale
+        rs = self._scal if self.state_bits == 32 else self.exp_avg_root_scale
+        ext().adamw_step(rows, chunks, kinds, m, r, ms, rs, self.step_count, self._scal,
+                         self._part, self._lr_t, self.betas[0], self.betas[1], self.eps,
+                         self.grad_clip)
+
+    # ---- CPU reference path (defines the kernels' semantics)
+
+    def _moment(self, name, off, n):
+        if self.state_bits == 32:
+            return getattr(self, name)[off:off + n].clone()
+        lo, hi = off // self.BLOCK, -(-(off + n) // self.BLOCK)
+        held = getattr(self, name)[lo * self.BLOCK:hi * self.BLOCK].float().view(-1, self.BLOCK)
+        return (held * getattr(self, name + "_scale")[lo:hi, None]).view(-1)[:n]
+
+    def _hold(self, name, off, n, value, least):
+        if self.state_bits == 32:
+            getattr(self, name)[off:off + n] = value
+            return
+        lo, hi = off // self.BLOCK, -(-(off + n) // self.BLOCK)
+        v = torch.zeros((hi - lo) * self.BLOCK)
+        v[:n] = value
+        v = v.view(-1, self.BLOCK)
+        finite = torch.nan_to_num(v.abs(), nan=0.0, posinf=math.inf)
+        top = finite.amax(1, keepdim=True).clamp_min(2.0 ** -100)
+        q = (v * (448.0 / top)).to(torch.float8_e4m3fn)
+        if least:
+            q = torch.where((v > 0) & (q.float() == 0), torch.tensor(2.0 ** -9), q.float()).to(torch.float8_e4m3fn)
+        getattr(self, name).view(torch.uint8)[lo * self.BLOCK:hi * self.BLOCK] = q.view(-1).view(torch.uint8)
+        getattr(self, name + "_scale")[lo:hi] = (top / 448.0).view(-1)
+
+    def _step_cpu(self):
+        (b1, b2), lr = self.betas, self.lr
+        views = self._views()
+        self.step_count += 1
+        t = int(self.step_count)
+        coef = 1.0
+        if self.grad_clip > 0:
+            sq = sum(float(g.double().square().sum()) for _, _, _, g, *_ in views if g is not None)
+            coef = min(1.0, self.grad_clip / (math.sqrt(sq) + 1e-6)) if sq == sq else math.nan
+        second = "exp_avg_sq" if self.state_bits == 32 else "exp_avg_root"
+        flat = lambda x: x.as_strided((x.numel(),), (1,))  # noqa: E731
+        for _, w, low, g, off, n, wd in views:
+            if g is None:
+                continue
+            gf = flat(g).float() * coef
+            m = b1 * self._moment("exp_avg", off, n) + (1 - b1) * gf
+            v = self._moment(second, off, n)
+            v = b2 * (v if self.state_bits == 32 else v.square()) + (1 - b2) * gf * gf
+            root = v.sqrt()
+            wf = flat(w)
+            wf.mul_(1 - lr * wd).sub_(lr * (m / (1 - b1 ** t)) / (root / math.sqrt(1 - b2 ** t) + self.eps))
+            if low is not None:
+                flat(low).copy_(wf)
+            self._hold("exp_avg", off, n, m, False)
+            self._hold(second, off, n, v if self.state_bits == 32 else root, True)
+
+    def state_dict(self):
+        sd = {"step": int(self.step_count), "lr": self.lr, "state_bits": self.state_bits}
+        sd.update({n: getattr(self, n) for n in self._names})
+        if self.flat is None and any(m is not None for m in self.masters):
+            sd["masters"] = self.masters
+        return sd
+
+    @torch.no_grad()
+    def load_state_dict(self, sd):
+        bits = 32 if "exp_avg_sq" in sd else 8
+        if bits != self.state_bits:
+            raise ValueError(f"FusedAdamW: the state is held in {bits} bits, this optimizer's in {self.state_bits}")
+        for n in self._names:
+            if sd[n].shape != getattr(self, n).shape or sd[n].dtype != getattr(self, n).dtype:
+                raise ValueError(f"FusedAdamW: {n} has another shape or type than this optimizer's")
+        for n in self._names:
+            getattr(self, n).copy_(sd[n])
+        if self.flat is None and "masters" in sd:
+            for mine, theirs in zip(self.masters, sd["masters"]):
+                if mine is not None:
+                    mine.copy_(theirs)
+        self.step_count.fill_(int(sd["step"]))
+        self.lr = sd.get("lr", self.lr)
+        self.param_groups[0]["lr"] = self.lr
