@@ -338,6 +338,9 @@ def main():
     gather_table = None
     graph_dump = os.environ.get("FAA_BENCH_GRAPH_DUMP")
 
+    # captures are checked on this thread alone: the process group's watchdog
+    # thread asks events of warm-up collectives meanwhile, which a global
+    # check takes for a mistake (it ends the capture, and the process)
     def _mk_graph():
         g_ = torch.cuda.CUDAGraph()
         if graph_dump:
@@ -378,12 +381,12 @@ def main():
             ag_mode = os.environ.get("FAA_BENCH_AG", "1") == "1"
             ag_grads = None
             if ag_mode:
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                     loss_ag = gpu_fwd_loss()
                     ag_grads = torch.autograd.grad(loss_ag, flat.params,
                                                    allow_unused=True)
             else:
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                     gpu_fwd_bwd()
             # grads now live in the graph pool at replay-stable addresses
             base = flat.flat_param.data_ptr()
@@ -423,11 +426,11 @@ def main():
                 torch.cuda.synchronize()
                 graph = _mk_graph()
                 upload_next()
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                     flat_capture_body() if dist_in_graph else step_body()
         else:
             try:
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                     flat_capture_body() if dist_in_graph else step_body()
             except Exception as e:
                 if not distributed:
@@ -444,7 +447,7 @@ def main():
                     model._sync_enabled = False   # hooks stay out of capture
                 graph = _mk_graph()
                 upload_next()
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                     flat_capture_body()
 
     if graph_dump and graph is not None:

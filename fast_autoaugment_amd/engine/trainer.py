@@ -92,7 +92,9 @@ class _GraphedTrainStep:
         self.label_s = label.clone()
         _t.cuda.synchronize()
         g = _t.cuda.CUDAGraph()
-        with _t.cuda.graph(g):
+        # checked on this thread alone: a process group's watchdog thread may
+        # ask events of earlier collectives meanwhile
+        with _t.cuda.graph(g, capture_error_mode="thread_local"):
             if self.flip:
                 from ..ops.conv import conv_flip_all
                 conv_flip_all()
