@@ -1,0 +1,104 @@
+"""Group normalisation with an activation, for channels-last maps (csrc/groupnorm.hip).
+
+The counterpart of the fused BatchNorm+activation (ops/bnrelu.py) for networks
+without batch statistics: small batches, accumulated gradients, evaluation that
+is the same function as training.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import require_ext_for
+
+ACTS = {"none": 0, "relu": 1, "swish": 2}
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class GroupNormActFn(torch.autograd.Function):
+    """x: [N, pixels, C], contiguous."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        C = require_ext_for(x)
+        y, mean, rstd = C.group_norm_fwd(x, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.groups, ctx.act = groups, act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        C = require_ext_for(x)
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        dx, *grads = C.group_norm_bwd(dy.contiguous(), x, ctx.groups, weight, bias, mean, rstd,
+                                      ctx.act, need_w or need_b)
+        dw, db = grads if grads else (None, None)
+        return dx, dw if need_w else None, db if need_b else None, None, None, None
+
+
+def _check(x, num_groups, weight, bias, eps, act):
+    if act not in ACTS:
+        raise ValueError(f"group_norm_act: act={act!r} is none of {sorted(ACTS)}")
+    if x.dim() < 2:
+        raise ValueError("group_norm_act: x is [N, C, ...]")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"group_norm_act: x is fp32, bf16 or fp16, not {x.dtype}")
+    c = x.size(1)
+    if num_groups < 1 or c < 1 or c % num_groups:
+        raise ValueError(f"group_norm_act: {c} channels cannot be {num_groups} groups")
+    if not eps >= 0.0:
+        raise ValueError("group_norm_act: eps >= 0 is needed")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.shape != (c,):
+            raise ValueError(f"group_norm_act: {name} is [{c}], not {list(p.shape)}")
+        if p.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"group_norm_act: {name} is of x's type or fp32, not {p.dtype}")
+        if p.device != x.device:
+            raise ValueError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError("group_norm_act: weight and bias are of one type")
+
+
+def _composed(x, num_groups, weight, bias, eps, act):
+    """The CPU path, which also defines the kernels' semantics."""
+    z = x.float()
+    if x.numel():
+        z = z.reshape(x.size(0), num_groups, -1)
+        z = z - z.mean(2, keepdim=True)
+        z = (z * (z.square().mean(2, keepdim=True) + eps).rsqrt()).reshape(x.shape)
+    column = (1, -1) + (1,) * (x.dim() - 2)
+    if weight is not None:
+        z = z * weight.float().view(column)
+    if bias is not None:
+        z = z + bias.float().view(column)
+    z = F.relu(z) if act == "relu" else F.silu(z) if act == "swish" else z
+    return z.to(x.dtype)
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                   act: str = "none") -> torch.Tensor:
+    """act(weight * (x - mean) / sqrt(var + eps) + bias), statistics over groups of channels.
+
+    x: [N, C, ...] in fp32, bf16 or fp16; mean and variance (biased) are taken
+    for each sample over the C / num_groups channels of a group and all pixels.
+    ``weight`` and ``bias`` are [C] or None, in x's type or fp32. ``act`` is
+    "none", "relu" or "swish". Everything is computed in fp32 and rounded once.
+    On the GPU the result is channels last (a map of another order is copied
+    into it first), and gradients go to x, weight and bias, once.
+    """
+    _check(x, num_groups, weight, bias, eps, act)
+    if not x.is_cuda:
+        return _composed(x, num_groups, weight, bias, eps, act)
+    rows = x.movedim(1, -1)
+    flat = rows.reshape(x.size(0), -1, x.size(1)) if x.numel() else rows.reshape(x.size(0), 0, x.size(1))
+    y = GroupNormActFn.apply(flat.contiguous(), None if weight is None else weight.contiguous(),
+                             None if bias is None else bias.contiguous(), num_groups, eps, ACTS[act])
+    return y.view(rows.shape).movedim(-1, 1)
