@@ -47,6 +47,8 @@ std::vector<torch::Tensor> group_norm_bwd(torch::Tensor dy, torch::Tensor x, int
                                           c10::optional<torch::Tensor> weight,
                                           c10::optional<torch::Tensor> bias, torch::Tensor mean,
                                           torch::Tensor rstd, int64_t act, bool param_grads);
+torch::Tensor linear_act(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> bias,
+                         c10::optional<torch::Tensor> residual, int64_t act);
 std::vector<torch::Tensor> residual_add_bn_stats(torch::Tensor a, torch::Tensor b);
 std::vector<torch::Tensor> bn_relu_bwd(torch::Tensor dy, torch::Tensor x,
                                        torch::Tensor out, torch::Tensor mean,
@@ -104,6 +106,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "out = a + b, plus BN fwd-reduce partials for the following bn");
   m.def("group_norm_fwd", &group_norm_fwd, "group norm + activation, [N, pixels, C]");
   m.def("group_norm_bwd", &group_norm_bwd);
+  m.def("linear_act", &linear_act, "act(x W^T + bias + residual), differentiable once");
   m.def("conv2d_fwd", &conv2d_fwd, "MFMA implicit-GEMM NHWC bf16 conv forward");
   m.def("conv2d_bwd_data", &conv2d_bwd_data);
   m.def("conv2d_bwd_data_s2", &conv2d_bwd_data_s2,

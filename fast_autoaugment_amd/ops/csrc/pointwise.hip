@@ -1,0 +1,708 @@
+// Matrix products with bias, residual and activation in their epilogue, and their gradients.
+//
+//   y  = act(z),  z = x W^T + b + r           x [M,K], W [N,K], b [N], r [M,N]
+//   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum dz,  dr = dz
+//
+// One kernel computes D[m][n] = sum_k P(m,k) Q(n,k) for 16-bit types, where each
+// operand lies either with k contiguous (x and W forward) or with its rows
+// contiguous (W for dx; dz and x for dW): no transposed copy is made. A
+// workgroup of 4 waves owns a BM x BN tile, steps through k by 64, and has the
+// next step's loads in flight in registers while it multiplies out of LDS.
+// Operands with contiguous rows are turned on their way out of LDS
+// (ds_read_b64_tr_b16). The roles in the matrix instruction are swapped (its
+// rows are n), so that a lane ends with 4 neighbouring columns of one output
+// row: 8-byte loads of the residual and stores of the result.
+//
+// A long k with few output tiles (dW: k is the batch's pixels) is split over
+// workgroups; parts go to a workspace in fp32 and are added in a fixed order by
+// a second kernel, which also has the epilogue.
+
+#include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include <hip/hip_fp16.h>
+#include "faa_common.h"
+
+namespace {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SWISH = 2, ACT_SIGMOID = 3 };
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+
+constexpr int BK = 64;
+
+// ------------------------------------------------------------ types
+
+template <typename T> struct Num;
+template <> struct Num<float> {
+  static __device__ __forceinline__ float get(const float* p) { return *p; }
+  static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
+template <> struct Num<__hip_bfloat16> {
+  typedef __hip_bfloat16 T;
+  static __device__ __forceinline__ float get(const T* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void put(T* p, float v) { *p = __float2bfloat16(v); }
+  static __device__ __forceinline__ float of(short u) { return __uint_as_float((uint32_t)(uint16_t)u << 16); }
+  static __device__ __forceinline__ short bits(float v) {
+    __hip_bfloat16 h = __float2bfloat16(v);
+    return *(short*)&h;
+  }
+  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Num<__half> {
+  typedef __half T;
+  static __device__ __forceinline__ float get(const T* p) { return __half2float(*p); }
+  static __device__ __forceinline__ void put(T* p, float v) { *p = __float2half(v); }
+  static __device__ __forceinline__ float of(short u) { return __half2float(__ushort_as_half((unsigned short)u)); }
+  static __device__ __forceinline__ short bits(float v) { return (short)__half_as_ushort(__float2half(v)); }
+  static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+
+// 4 neighbours of a row that has `left` of them
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* p, int left, bool vec) {
+  f32x4 v = {0, 0, 0, 0};
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      v = *(const f32x4*)p;
+    } else {
+      s16x4 u = *(const s16x4*)p;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = Num<T>::of(u[i]);
+    }
+    return v;
+  }
+  #pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left) v[i] = Num<T>::get(p + i);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int left, bool vec, f32x4 v) {
+  if (vec && left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *(f32x4*)p = v;
+    } else {
+      s16x4 u;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = Num<T>::bits(v[i]);
+      *(s16x4*)p = u;
+    }
+    return;
+  }
+  #pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < left) Num<T>::put(p + i, v[i]);
+}
+
+__device__ __forceinline__ float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+}
+__device__ __forceinline__ float act_value(float z, int act) {
+  if (act == ACT_RELU) return z < 0.0f ? 0.0f : z;      // a NaN stays one
+  if (act == ACT_SWISH) return z * sigmoid(z);
+  if (act == ACT_SIGMOID) return sigmoid(z);
+  return z;
+}
+// from z, or for relu from y: both are above 0 in the same places
+__device__ __forceinline__ float act_slope(float z, int act) {
+  if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  const float s = sigmoid(z);
+  if (act == ACT_SWISH) return s * (1.0f + z * (1.0f - s));
+  if (act == ACT_SIGMOID) return s * (1.0f - s);
+  return 1.0f;
+}
+
+// ------------------------------------------------------------ epilogue
+
+template <typename T>
+struct Epilogue {
+  const T* bias;      // [N] or null
+  const T* res;       // [M,N] or null
+  T* y;               // [M,N]
+  T* z;               // [M,N] or null: the sum before the activation, for the backward pass
+  int act;
+  bool vec;           // rows of 4 may be read and written at once
+
+  __device__ __forceinline__ void operator()(int64_t m, int n, int N, f32x4 v) const {
+    const int left = N - n;
+    if (left <= 0) return;
+    const int64_t at = m * N + n;
+    if (bias) v += load4(bias + n, left, vec);
+    if (res) v += load4(res + at, left, vec);
+    if (z) {
+      store4(z + at, left, vec, v);
+      // the backward pass has z in its own type; y is that of the exact sum
+    }
+    if (act != ACT_NONE) {
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], act);
+    }
+    store4(y + at, left, vec, v);
+  }
+};
+
+// ------------------------------------------------------------ operands
+
+// P(row, k): row-major with k contiguous, or (ROWS) k-major with rows contiguous
+template <typename T>
+struct Operand {
+  const T* p;
+  int rows, kdim;
+  int64_t ld;
+  bool vec;           // 8 neighbours may be loaded at once, and none of them lies over the edge
+};
+
+template <typename T, bool ROWS>
+__device__ __forceinline__ s16x8 load8(const Operand<T>& o, int row, int k) {
+  s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (ROWS ? k >= o.kdim : row >= o.rows) return v;
+  const T* p = ROWS ? o.p + (int64_t)k * o.ld + row : o.p + (int64_t)row * o.ld + k;
+  const int left = ROWS ? o.rows - row : o.kdim - k;
+  if (o.vec) {
+    if (left > 0) v = *(const s16x8*)p;
+  } else {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) v[i] = *(const short*)(p + i);
+  }
+  return v;
+}
+
+// A tile of B rows and 64 k in LDS, 16 bytes a piece.
+// k contiguous: row r has 8 pieces, piece q at q ^ (r & 7): 8 lanes that read one q of 8 rows meet 8 places.
+// rows contiguous: line k has B/8 pieces. The transposing read of one instruction touches lines
+// {0..3} + 8g (g = 0..3), 32 bytes of each: pairs of pieces are moved by the line so that these lie apart.
+template <int B, bool ROWS>
+struct Lds {
+  static constexpr int kPieces = B * BK / 8;
+  static __device__ __forceinline__ void place(int c, int& row, int& k) {
+    if (ROWS) { k = c / (B / 8); row = (c % (B / 8)) * 8; }
+    else { row = c / 8; k = (c % 8) * 8; }
+  }
+  static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 1) & 4)) & (B / 16 - 1); }
+  static __device__ __forceinline__ int at(int c) {     // in shorts
+    if (ROWS) {
+      const int k = c / (B / 8), p = c % (B / 8);
+      return k * B + (((p >> 1) ^ turn(k)) * 2 + (p & 1)) * 8;
+    }
+    const int row = c / 8, q = c % 8;
+    return row * BK + ((q ^ (row & 7)) * 8);
+  }
+  // fragment of 16 rows from row0, 32 k from k0: lane has row lane%16, k (lane/16)*8 .. +7
+  static __device__ __forceinline__ s16x8 fragment(short* lds, int row0, int k0, int lane) {
+    if (!ROWS) {
+      const int row = row0 + (lane & 15), q = k0 / 8 + (lane >> 4);
+      return *(const s16x8*)(lds + row * BK + ((q ^ (row & 7)) * 8));
+    }
+    const int i = lane & 15, k = k0 + (lane >> 4) * 8 + (i >> 2);
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    auto word = [&](int kk) {
+      return lds + kk * B + ((row0 / 16) ^ turn(kk)) * 16 + (i & 3) * 4;
+    };
+    s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)word(k));
+    s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)word(k + 4));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+// Workgroups that share operand rows run one after another on one XCD and find them in its L2.
+__device__ __forceinline__ int xcd_order(int wg, int n) {
+  const int q = n / 8, rem = n % 8, xcd = wg % 8, i = wg / 8;
+  return xcd < rem ? xcd * (q + 1) + i : rem * (q + 1) + (xcd - rem) * q + i;
+}
+
+// ------------------------------------------------------------ the product in 16 bits
+
+template <typename T, bool PR, bool QR, int BM, int BN>
+__global__ __launch_bounds__(256) void product_kernel(Operand<T> P, Operand<T> Q, Epilogue<T> epi,
+                                                      float* __restrict__ part, int tiles_m,
+                                                      int tiles_n, int splits) {
+  constexpr int FM = BM / 32, FN = BN / 32;         // fragments of a wave: 2 x 2 waves
+  constexpr int NP = Lds<BM, PR>::kPieces / 256, NQ = Lds<BN, QR>::kPieces / 256;
+  __shared__ __align__(16) short lds_p[2][BM * BK];
+  __shared__ __align__(16) short lds_q[2][BN * BK];
+  const int id = xcd_order((int)blockIdx.x, tiles_m * tiles_n * splits);
+  const int tn = id % tiles_n, tm = id / tiles_n % tiles_m, sp = id / tiles_n / tiles_m;
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int steps = (P.kdim + BK - 1) / BK;
+  const int s0 = (int)((int64_t)steps * sp / splits), s1 = (int)((int64_t)steps * (sp + 1) / splits);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
+
+  s16x8 rp[NP], rq[NQ];
+  auto fetch = [&](int s) {
+    #pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      int row, k;
+      Lds<BM, PR>::place(tid + i * 256, row, k);
+      rp[i] = load8<T, PR>(P, m0 + row, s * BK + k);
+    }
+    #pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      int row, k;
+      Lds<BN, QR>::place(tid + i * 256, row, k);
+      rq[i] = load8<T, QR>(Q, n0 + row, s * BK + k);
+    }
+  };
+  auto put = [&](int buf) {
+    #pragma unroll
+    for (int i = 0; i < NP; ++i) *(s16x8*)(lds_p[buf] + Lds<BM, PR>::at(tid + i * 256)) = rp[i];
+    #pragma unroll
+    for (int i = 0; i < NQ; ++i) *(s16x8*)(lds_q[buf] + Lds<BN, QR>::at(tid + i * 256)) = rq[i];
+  };
+
+  f32x4 acc[FM][FN];
+  #pragma unroll
+  for (int i = 0; i < FM; ++i)
+    #pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  if (s0 < s1) {
+    fetch(s0);
+    put(0);
+    if (s0 + 1 < s1) fetch(s0 + 1);
+  }
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    const int buf = (s - s0) & 1;
+    if (s + 1 < s1) {
+      put(buf ^ 1);                       // its readers are behind the last barrier
+      if (s + 2 < s1) fetch(s + 2);
+    }
+    #pragma unroll
+    for (int k = 0; k < BK; k += 32) {
+      s16x8 fp[FM], fq[FN];
+      #pragma unroll
+      for (int i = 0; i < FM; ++i) fp[i] = Lds<BM, PR>::fragment(lds_p[buf], wm + i * 16, k, lane);
+      #pragma unroll
+      for (int j = 0; j < FN; ++j) fq[j] = Lds<BN, QR>::fragment(lds_q[buf], wn + j * 16, k, lane);
+      #pragma unroll
+      for (int i = 0; i < FM; ++i)
+        #pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
+    }
+    __syncthreads();
+  }
+  // lane: output row lane%16 of a fragment, columns (lane/16)*4 .. +3
+  const int M = P.rows, N = Q.rows;
+  #pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int64_t m = (int64_t)m0 + wm + i * 16 + (lane & 15);
+    if (m >= M) continue;
+    #pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+      if (splits == 1) epi(m, n, N, acc[i][j]);
+      else if (n < N) store4(part + ((int64_t)sp * M + m) * N + n, N - n, epi.vec, acc[i][j]);
+    }
+  }
+}
+
+// ------------------------------------------------------------ the product in 32 bits
+
+// 64 x 64 tiles, 16 k a step; LDS lines hold one k (a lane of the matrix instruction has one k of one row)
+template <bool PR, bool QR>
+__global__ __launch_bounds__(256) void product_f32_kernel(Operand<float> P, Operand<float> Q,
+                                                          Epilogue<float> epi, float* __restrict__ part,
+                                                          int tiles_m, int tiles_n, int splits) {
+  constexpr int B = 64, K = 16, LD = B + 4;
+  __shared__ float lp[2][K][LD], lq[2][K][LD];
+  const int id = xcd_order((int)blockIdx.x, tiles_m * tiles_n * splits);
+  const int tn = id % tiles_n, tm = id / tiles_n % tiles_m, sp = id / tiles_n / tiles_m;
+  const int m0 = tm * B, n0 = tn * B;
+  const int steps = (P.kdim + K - 1) / K;
+  const int s0 = (int)((int64_t)steps * sp / splits), s1 = (int)((int64_t)steps * (sp + 1) / splits);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+  float rp[4], rq[4];
+  auto one = [](const Operand<float>& o, bool rows, int row, int k) {
+    if (row >= o.rows || k >= o.kdim) return 0.0f;
+    return rows ? o.p[(int64_t)k * o.ld + row] : o.p[(int64_t)row * o.ld + k];
+  };
+  auto place = [&](bool rows, int i, int& row, int& k) {
+    const int c = tid + i * 256;
+    if (rows) { k = c / B; row = c % B; }
+    else { row = c / K; k = c % K; }
+  };
+  auto fetch = [&](int s) {
+    int row, k;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      place(PR, i, row, k);
+      rp[i] = one(P, PR, m0 + row, s * K + k);
+      place(QR, i, row, k);
+      rq[i] = one(Q, QR, n0 + row, s * K + k);
+    }
+  };
+  auto put = [&](int buf) {
+    int row, k;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      place(PR, i, row, k);
+      lp[buf][k][row] = rp[i];
+      place(QR, i, row, k);
+      lq[buf][k][row] = rq[i];
+    }
+  };
+  f32x4 acc[2][2];
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0, 0, 0, 0};
+  if (s0 < s1) {
+    fetch(s0);
+    put(0);
+    if (s0 + 1 < s1) fetch(s0 + 1);
+  }
+  __syncthreads();
+  for (int s = s0; s < s1; ++s) {
+    const int buf = (s - s0) & 1;
+    if (s + 1 < s1) {
+      put(buf ^ 1);
+      if (s + 2 < s1) fetch(s + 2);
+    }
+    #pragma unroll
+    for (int k = 0; k < K; k += 4) {
+      float fp[2], fq[2];
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fp[i] = lp[buf][k + (lane >> 4)][wm + i * 16 + (lane & 15)];
+        fq[i] = lq[buf][k + (lane >> 4)][wn + i * 16 + (lane & 15)];
+      }
+      #pragma unroll
+      for (int i = 0; i < 2; ++i)
+        #pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fq[j], fp[i], acc[i][j], 0, 0, 0);
+    }
+    __syncthreads();
+  }
+  const int M = P.rows, N = Q.rows;
+  #pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t m = (int64_t)m0 + wm + i * 16 + (lane & 15);
+    if (m >= M) continue;
+    #pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+      if (splits == 1) epi(m, n, N, acc[i][j]);
+      else if (n < N) store4(part + ((int64_t)sp * M + m) * N + n, N - n, epi.vec, acc[i][j]);
+    }
+  }
+}
+
+// the parts of a split product, added in order, and its epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ part, Epilogue<T> epi,
+                                                   int64_t M, int N, int splits) {
+  const int n4 = (N + 3) / 4;
+  const int64_t total = M * n4, plane = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / n4;
+    const int n = (int)(i - m * n4) * 4;
+    f32x4 v = {0, 0, 0, 0};
+    for (int s = 0; s < splits; ++s) v += load4(part + s * plane + m * N + n, N - n, epi.vec);
+    epi(m, n, N, v);
+  }
+}
+
+// ------------------------------------------------------------ dz and its column sums
+
+// dz = dy act'(z) where dz is given; sums over a chunk of rows to part[chunk][N] where part is given.
+// A thread has VEC columns, a workgroup a tile of columns and a chunk of rows.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ z,
+                                                    T* __restrict__ dz, float* __restrict__ part,
+                                                    int64_t M, int N, int tile, int ntile, int chunk,
+                                                    int act) {
+  __shared__ float lds[256 * VEC];
+  const int64_t wg = blockIdx.x;
+  const int ti = (int)(wg % ntile);
+  const int64_t ck = wg / ntile;
+  const int c0 = ti * tile, cols = min(tile, N - c0), cv = cols / VEC, rows = 256 / cv;
+  const int r = (int)threadIdx.x / cv, v = (int)threadIdx.x - r * cv;
+  const bool on = r < rows;
+  const int64_t m0 = ck * chunk, m1 = min(m0 + chunk, M);
+  float acc[VEC];
+  #pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+  if (on) {
+    #pragma unroll 4
+    for (int64_t m = m0 + r; m < m1; m += rows) {
+      const int64_t at = m * N + c0 + v * VEC;
+      if constexpr (VEC == 1) {
+        float d = Num<T>::get(dy + at);
+        if (dz) {
+          d *= act_slope(Num<T>::get(z + at), act);
+          Num<T>::put(dz + at, d);
+        }
+        acc[0] += d;
+      } else {
+        constexpr int H = VEC / 4;
+        f32x4 d[H], zz[H];
+        #pragma unroll
+        for (int h = 0; h < H; ++h) {
+          d[h] = load4(dy + at + 4 * h, 4, true);
+          if (dz) zz[h] = load4(z + at + 4 * h, 4, true);
+        }
+        #pragma unroll
+        for (int h = 0; h < H; ++h) {
+          if (dz) {
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) d[h][i] *= act_slope(zz[h][i], act);
+            store4(dz + at + 4 * h, 4, true, d[h]);
+          }
+          #pragma unroll
+          for (int i = 0; i < 4; ++i) acc[4 * h + i] += d[h][i];
+        }
+      }
+    }
+  }
+  if (!part) return;
+  if (on)
+    #pragma unroll
+    for (int j = 0; j < VEC; ++j) lds[r * cols + v * VEC + j] = acc[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < cols; c += 256) {
+    float s = 0.0f;
+    for (int q = 0; q < rows; ++q) s += lds[q * cols + c];
+    part[ck * N + c0 + c] = s;
+  }
+}
+
+// out[n] = sum over the chunks, 32 columns a workgroup
+template <typename T>
+__global__ __launch_bounds__(1024) void column_join_kernel(const float* __restrict__ part, int64_t chunks,
+                                                           int N, T* __restrict__ out) {
+  __shared__ float lds[32][33];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
+  float s = 0.0f;
+  if (n < N)
+    for (int64_t r = row; r < chunks; r += 32) s += part[r * N + n];
+  lds[row][col] = s;
+  __syncthreads();
+  if (row == 0 && n < N) {
+    s = 0.0f;
+    #pragma unroll
+    for (int r = 0; r < 32; ++r) s += lds[r][col];
+    Num<T>::put(out + n, s);
+  }
+}
+
+// ------------------------------------------------------------ host
+
+bool aligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+template <typename F>
+void by_type(torch::ScalarType t, F f) {
+  if (t == torch::kFloat32) f(float{});
+  else if (t == torch::kBFloat16) f(__hip_bfloat16{});
+  else if (t == torch::kFloat16) f(__half{});
+  else TORCH_CHECK(false, "linear_act: fp32, bf16 and fp16 are taken");
+}
+
+template <typename T>
+Operand<T> operand(const torch::Tensor& t, bool rows_contiguous) {
+  Operand<T> o;
+  o.p = (const T*)t.data_ptr();
+  o.rows = (int)t.size(rows_contiguous ? 1 : 0);
+  o.kdim = (int)t.size(rows_contiguous ? 0 : 1);
+  o.ld = t.size(1);
+  o.vec = t.size(1) % 8 == 0 && aligned(o.p, 16);
+  return o;
+}
+
+// D[m][n] = sum_k P(m,k) Q(n,k), with the epilogue
+template <typename T, bool PR, bool QR>
+void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hipStream_t stream) {
+  const Operand<T> P = operand<T>(p, PR), Q = operand<T>(q, QR);
+  const int64_t M = P.rows, N = Q.rows, K = P.kdim;
+  epi.vec = N % 4 == 0 && aligned(epi.y, 4 * sizeof(T)) && (!epi.z || aligned(epi.z, 4 * sizeof(T)))
+            && (!epi.res || aligned(epi.res, 4 * sizeof(T)))
+            && (!epi.bias || aligned(epi.bias, 4 * sizeof(T)));
+  int BM = 64, BN = 64, step = 16;
+  if constexpr (sizeof(T) == 2) {
+    step = BK;
+    auto tiles = [&](int64_t a, int64_t b) { return ((M + a - 1) / a) * ((N + b - 1) / b); };
+    if (M > 64 && tiles(128, 64) >= 256) BM = 128;
+    if (BM == 128 && N > 64 && tiles(128, 128) >= 256) BN = 128;
+  }
+  const int64_t tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, steps = (K + step - 1) / step;
+  // few tiles and a long k: enough parts for 2 workgroups a CU, each with 4 steps at least
+  int64_t splits = 1;
+  if (tm * tn < 256) splits = std::max<int64_t>(1, std::min<int64_t>(512 / (tm * tn), steps / 4));
+  TORCH_CHECK(tm * tn * splits < (int64_t(1) << 31), "linear_act: too many tiles");
+  torch::Tensor ws;
+  float* part = nullptr;
+  if (splits > 1) {
+    ws = torch::empty({splits * M * N}, p.options().dtype(torch::kFloat32));
+    part = ws.data_ptr<float>();
+  }
+  const dim3 grid((unsigned)(tm * tn * splits)), block(256);
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, block, 0, stream, P, Q, epi, part, (int)tm, (int)tn, (int)splits);
+  };
+  if constexpr (sizeof(T) == 4) {
+    go(product_f32_kernel<PR, QR>);
+  } else if (BM == 128 && BN == 128) {
+    go(product_kernel<T, PR, QR, 128, 128>);
+  } else if (BM == 128) {
+    go(product_kernel<T, PR, QR, 128, 64>);
+  } else {
+    go(product_kernel<T, PR, QR, 64, 64>);
+  }
+  if (splits > 1) {
+    const int64_t work = M * ((N + 3) / 4);
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)std::min<int64_t>((work + 255) / 256, 4096)),
+                       dim3(256), 0, stream, part, epi, M, (int)N, (int)splits);
+  }
+}
+
+template <typename T>
+void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, torch::Tensor* db, int act,
+           hipStream_t stream) {
+  const int64_t M = dy.size(0);
+  const int N = (int)dy.size(1);
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = N % V == 0 && aligned(dy.data_ptr(), 16) && (!dz || (aligned(dz->data_ptr(), 16)
+                   && aligned(z->data_ptr(), 16)));
+  const int vw = vec ? V : 1, tile = std::min(N, (vec ? 32 : 64) * vw), ntile = (N + tile - 1) / tile;
+  const int rows = 256 / (tile / vw);
+  // about 2048 workgroups, and chunks of 8 rows a thread at least
+  int64_t chunk = std::max<int64_t>(8, (M * ntile / 2048 + rows - 1) / rows) * rows;
+  chunk = std::min<int64_t>(chunk, 1 << 24);
+  const int64_t chunks = (M + chunk - 1) / chunk;
+  TORCH_CHECK(chunks * ntile < (int64_t(1) << 31), "linear_act: too many rows");
+  torch::Tensor ws;
+  if (db) ws = torch::empty({chunks * N}, dy.options().dtype(torch::kFloat32));
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)(chunks * ntile)), dim3(256), 0, stream,
+                       (const T*)dy.data_ptr(), z ? (const T*)z->data_ptr() : nullptr,
+                       dz ? (T*)dz->data_ptr() : nullptr, db ? ws.data_ptr<float>() : nullptr, M, N, tile,
+                       ntile, (int)chunk, act);
+  };
+  if (vec) go(slope_kernel<T, V>);
+  else go(slope_kernel<T, 1>);
+  if (db)
+    hipLaunchKernelGGL((column_join_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, stream,
+                       ws.data_ptr<float>(), chunks, N, (T*)db->data_ptr());
+}
+
+void check(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& b, const torch::Tensor& r,
+           int64_t act) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 && x.is_contiguous() && w.is_contiguous(),
+              "linear_act: x [M,K] and weight [N,K], contiguous");
+  TORCH_CHECK(x.size(1) == w.size(1) && x.size(1) > 0 && w.size(0) > 0, "linear_act: sizes");
+  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 256 && x.size(1) < (1 << 30) && w.size(0) < (1 << 30),
+              "linear_act: a dimension is too large");
+  TORCH_CHECK(w.scalar_type() == x.scalar_type() && w.device() == x.device(), "linear_act: weight");
+  TORCH_CHECK(!b.defined() || (b.is_contiguous() && b.dim() == 1 && b.size(0) == w.size(0)
+              && b.scalar_type() == x.scalar_type() && b.device() == x.device()), "linear_act: bias");
+  TORCH_CHECK(!r.defined() || (r.is_contiguous() && r.dim() == 2 && r.size(0) == x.size(0)
+              && r.size(1) == w.size(0) && r.scalar_type() == x.scalar_type()
+              && r.device() == x.device()), "linear_act: residual");
+  TORCH_CHECK(act >= 0 && act <= 3, "linear_act: activation");
+}
+
+class LinearAct : public torch::autograd::Function<LinearAct> {
+ public:
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor x, torch::Tensor w,
+                               c10::optional<torch::Tensor> bias, c10::optional<torch::Tensor> res,
+                               int64_t act, bool train) {
+    const auto b = bias.value_or(torch::Tensor()), r = res.value_or(torch::Tensor());
+    check(x, w, b, r, act);
+    const c10::OptionalDeviceGuard guard(x.device());
+    auto stream = at::hip::getCurrentHIPStream().stream();
+    auto y = torch::empty({x.size(0), w.size(0)}, x.options());
+    const bool keep = train && (act == ACT_SWISH || act == ACT_SIGMOID);
+    auto z = keep ? torch::empty_like(y) : torch::Tensor();
+    if (x.size(0) > 0)
+      by_type(x.scalar_type(), [&](auto t) {
+        using T = decltype(t);
+        Epilogue<T> epi{b.defined() ? (const T*)b.data_ptr() : nullptr,
+                        r.defined() ? (const T*)r.data_ptr() : nullptr, (T*)y.data_ptr(),
+                        keep ? (T*)z.data_ptr() : nullptr, (int)act, false};
+        product<T, false, false>(x, w, epi, stream);
+      });
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = b.defined();
+    ctx->saved_data["res"] = r.defined();
+    // relu's slope is known from its result
+    ctx->save_for_backward({x, w, keep ? z : act == ACT_RELU ? y : torch::Tensor()});
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &w = saved[1], &z = saved[2];
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const c10::OptionalDeviceGuard guard(x.device());
+    auto stream = at::hip::getCurrentHIPStream().stream();
+    // absent tensors are not counted among the inputs
+    const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["res"].toBool();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1),
+               nb = has_b && ctx->needs_input_grad(2), nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+    torch::Tensor dy, dz, dx, dw, db;
+    const int64_t M = x.size(0), N = w.size(0);
+    const bool again = at::GradMode::is_enabled();
+    {
+      at::NoGradGuard off;
+      dy = grads[0].contiguous();
+      if (nb) db = torch::empty({N}, x.options());
+      if (nx) dx = torch::empty_like(x);
+      if (nw) dw = torch::empty_like(w);
+      dz = act == ACT_NONE ? dy : torch::empty_like(dy);
+      if (M == 0) {
+        if (nb) db.zero_();
+        if (nw) dw.zero_();
+      } else {
+        by_type(x.scalar_type(), [&](auto t) {
+          using T = decltype(t);
+          if (act != ACT_NONE || nb)
+            slope<T>(dy, act == ACT_NONE ? nullptr : &z, act == ACT_NONE ? nullptr : &dz,
+                     nb ? &db : nullptr, act, stream);
+          Epilogue<T> epi{nullptr, nullptr, nullptr, nullptr, ACT_NONE, false};
+          if (nx) {
+            epi.y = (T*)dx.data_ptr();
+            product<T, false, true>(dz, w, epi, stream);
+          }
+          if (nw) {
+            epi.y = (T*)dw.data_ptr();
+            product<T, true, true>(dz, x, epi, stream);
+          }
+        });
+      }
+    }
+    torch::autograd::variable_list out{dx, dw, db, nr ? dz : torch::Tensor(), torch::Tensor(),
+                                       torch::Tensor()};
+    if (again)      // differentiating these again is an error, not a zero
+      for (auto& g : out)
+        if (g.defined()) {
+          auto err = std::make_shared<torch::autograd::DelayedError>(
+              "linear_act is differentiable once", 1);
+          g = (*err)({g.detach().requires_grad_(true)})[0];
+        }
+    return out;
+  }
+};
+
+}  // namespace
+
+torch::Tensor linear_act(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> bias,
+                         c10::optional<torch::Tensor> residual, int64_t act) {
+  const bool train = at::GradMode::is_enabled()
+                     && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad())
+                         || (residual && residual->requires_grad()));
+  return LinearAct::apply(x, weight, bias, residual, act, train);
+}

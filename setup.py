@@ -24,8 +24,10 @@ sources = [
     os.path.join(CSRC, "adamw.hip"),
     os.path.join(CSRC, "aug_kernels.hip"),
     os.path.join(CSRC, "bnrelu.hip"),
+    os.path.join(CSRC, "groupnorm.hip"),
     os.path.join(CSRC, "conv_mfma.hip"),
     os.path.join(CSRC, "depthwise.hip"),
+    os.path.join(CSRC, "pointwise.hip"),
 ]
 
 setup(
