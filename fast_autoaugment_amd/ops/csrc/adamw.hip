@@ -25,6 +25,7 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <hip/hip_fp16.h>
 #include "faa_common.h"
 
@@ -349,4 +350,5 @@ void adamw_step(std::vector<torch::Tensor> rows, std::vector<torch::Tensor> chun
     else
       launch_step<__half, true>(rows[i], chunks[i], st, bits, s, l, b1, b2, eps, stream);
   }
+  C10_HIP_KERNEL_LAUNCH_CHECK();
 }

@@ -40,13 +40,8 @@ std::vector<torch::Tensor> bn_relu_fwd(torch::Tensor x, torch::Tensor gamma,
                                        torch::Tensor running_var, bool training,
                                        double momentum, double eps, int64_t act,
                                        torch::Tensor pre_scratch);
-std::vector<torch::Tensor> group_norm_fwd(torch::Tensor x, int64_t groups,
-                                          c10::optional<torch::Tensor> weight,
-                                          c10::optional<torch::Tensor> bias, double eps, int64_t act);
-std::vector<torch::Tensor> group_norm_bwd(torch::Tensor dy, torch::Tensor x, int64_t groups,
-                                          c10::optional<torch::Tensor> weight,
-                                          c10::optional<torch::Tensor> bias, torch::Tensor mean,
-                                          torch::Tensor rstd, int64_t act, bool param_grads);
+torch::Tensor group_norm_act(torch::Tensor x, int64_t groups, c10::optional<torch::Tensor> weight,
+                             c10::optional<torch::Tensor> bias, double eps, int64_t act);
 torch::Tensor linear_act(torch::Tensor x, torch::Tensor weight, c10::optional<torch::Tensor> bias,
                          c10::optional<torch::Tensor> residual, int64_t act);
 std::vector<torch::Tensor> residual_add_bn_stats(torch::Tensor a, torch::Tensor b);
@@ -104,8 +99,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bn_relu_fwd", &bn_relu_fwd);
   m.def("residual_add_bn_stats", &residual_add_bn_stats,
         "out = a + b, plus BN fwd-reduce partials for the following bn");
-  m.def("group_norm_fwd", &group_norm_fwd, "group norm + activation, [N, pixels, C]");
-  m.def("group_norm_bwd", &group_norm_bwd);
+  m.def("group_norm_act", &group_norm_act, "group norm + activation, differentiable once");
   m.def("linear_act", &linear_act, "act(x W^T + bias + residual), differentiable once");
   m.def("conv2d_fwd", &conv2d_fwd, "MFMA implicit-GEMM NHWC bf16 conv forward");
   m.def("conv2d_bwd_data", &conv2d_bwd_data);

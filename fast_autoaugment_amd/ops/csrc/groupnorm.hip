@@ -15,10 +15,13 @@
 // channels are joined to groups last, so a group may be any number of channels.
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <hip/hip_fp16.h>
 #include <numeric>
+#include <type_traits>
 #include "faa_common.h"
 
 namespace {
@@ -28,11 +31,6 @@ enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SWISH = 2 };
 // ------------------------------------------------------------ loads and stores
 
 template <typename T, int VEC> struct Pack;
-template <int VEC> struct Pack<float, VEC> {
-  typedef __attribute__((ext_vector_type(VEC))) float raw;
-  static __device__ __forceinline__ float get(const raw& r, int j) { return r[j]; }
-  static __device__ __forceinline__ void set(raw& r, int j, float v) { r[j] = v; }
-};
 template <> struct Pack<float, 1> {
   typedef float raw;
   static __device__ __forceinline__ float get(const raw& r, int) { return r; }
@@ -58,11 +56,31 @@ template <typename T> struct Pack<T, 8> {
   static __device__ __forceinline__ float get(const raw& r, int j) { return bits_to_float<T>(r[j]); }
   static __device__ __forceinline__ void set(raw& r, int j, float v) { r[j] = float_to_bits<T>(v); }
 };
+template <typename T> struct Pack<T, 4> {
+  typedef __attribute__((ext_vector_type(4))) unsigned short raw;
+  static __device__ __forceinline__ float get(const raw& r, int j) { return bits_to_float<T>(r[j]); }
+  static __device__ __forceinline__ void set(raw& r, int j, float v) { r[j] = float_to_bits<T>(v); }
+};
+template <> struct Pack<float, 4> {
+  typedef __attribute__((ext_vector_type(4))) float raw;
+  static __device__ __forceinline__ float get(const raw& r, int j) { return r[j]; }
+  static __device__ __forceinline__ void set(raw& r, int j, float v) { r[j] = v; }
+};
 template <typename T> struct Pack<T, 1> {
   typedef unsigned short raw;
   static __device__ __forceinline__ float get(const raw& r, int) { return bits_to_float<T>(r); }
   static __device__ __forceinline__ void set(raw& r, int, float v) { r = float_to_bits<T>(v); }
 };
+
+// VEC values `bytes` behind a base that is the same for a whole wave: one register of address a thread
+template <typename T, int VEC>
+__device__ __forceinline__ typename Pack<T, VEC>::raw load_at(const T* base, uint32_t bytes) {
+  return *(const typename Pack<T, VEC>::raw*)((const char*)base + bytes);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_at(T* base, uint32_t bytes, const typename Pack<T, VEC>::raw& v) {
+  *(typename Pack<T, VEC>::raw*)((char*)base + bytes) = v;
+}
 
 // weight or bias of channel c: absent, fp32, or the map's type
 template <typename T>
@@ -80,21 +98,31 @@ __device__ __forceinline__ float param<__half>(const void* p, bool f32, int c, f
   return f32 ? ((const float*)p)[c] : __half2float(((const __half*)p)[c]);
 }
 
+// exp2 without the range handling of expf: what it would give below 2^-126 is nothing next to 1
 __device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
-__device__ __forceinline__ float act_value(float z, int act) {
-  if (act == ACT_RELU) return z < 0.0f ? 0.0f : z;      // a NaN stays one
-  if (act == ACT_SWISH) return z * sigmoid(z);
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if (ACT == ACT_RELU) return z < 0.0f ? 0.0f : z;      // a NaN stays one
+  if (ACT == ACT_SWISH) return z * sigmoid(z);
   return z;
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (act == ACT_SWISH) {
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (ACT == ACT_SWISH) {
     const float s = sigmoid(z);
-    return s * (1.0f + z * (1.0f - s));
+    return s + s * (z - z * s);
   }
   return 1.0f;
+}
+// f(activation as a constant): one branch outside the loops, not one an element
+template <typename F>
+__device__ __forceinline__ void by_act(int act, F f) {
+  if (act == ACT_SWISH) f(std::integral_constant<int, ACT_SWISH>{});
+  else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  else f(std::integral_constant<int, ACT_NONE>{});
 }
 
 // ------------------------------------------------------------ sums in a workgroup
@@ -125,14 +153,14 @@ __device__ __forceinline__ void channel_sums(const Tile& t, const float (&acc)[K
   }
   __syncthreads();
   // several threads share a column while there are threads left, and leave their sums in the first rows
-  int share = (int)blockDim.x / t.ch;
-  share = share < 1 ? 1 : (share > t.rows ? t.rows : share);
+  int share = min(min((int)blockDim.x / t.ch, t.rows), 8);
   if (share > 1) {
     const int s = (int)threadIdx.x / t.ch, c = (int)threadIdx.x - s * t.ch;
     if (s < share) {
       #pragma unroll
       for (int k = 0; k < K; ++k) {
         float sum = 0.0f;
+        #pragma unroll 4
         for (int r = s; r < t.rows; r += share) sum += lds[k * plane + r * t.ch + c];
         lds[k * plane + s * t.ch + c] = sum;    // row s is this thread's own from here on
       }
@@ -144,10 +172,107 @@ __device__ __forceinline__ void channel_sums(const Tile& t, const float (&acc)[K
   for (int i = threadIdx.x; i < K * t.ch; i += blockDim.x) {
     const int k = i / t.ch, c = i - k * t.ch;
     float sum = 0.0f;
+    #pragma unroll 4
     for (int r = 0; r < share; ++r) sum += lds[k * plane + r * t.ch + c];
     out[i] = sum;
   }
   __syncthreads();
+}
+
+// A channel's mean and sum of squares around it (out[c], out[ch+c]) from those of every thread's own pixels:
+// parts are moved to the common mean, so nothing large is subtracted. np: pixels of the tile, row r has
+// those r, r+rows, ... lds: 2*blockDim*VEC + 8 floats.
+template <int VEC>
+__device__ __forceinline__ void channel_moments(const Tile& t, const float (&mean)[VEC],
+                                                const float (&m2)[VEC], int np, float* lds, float* out) {
+  const int plane = (int)blockDim.x * VEC;
+  if (t.on) {
+    #pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      lds[t.r * t.ch + t.v * VEC + j] = mean[j];
+      lds[plane + t.r * t.ch + t.v * VEC + j] = m2[j];
+    }
+  }
+  __syncthreads();
+  const int full = np / t.rows, rem = np - full * t.rows, rows = min(t.rows, np);
+  const float inv_np = 1.0f / (float)np;
+  // rows first, first+by, ... to (mean, m2); their pixels are returned
+  auto join = [&](int first, int by, int c, float& mean_o, float& m2_o) {
+    float s = 0.0f, n = 0.0f, q = 0.0f;
+    #pragma unroll 4
+    for (int r = first; r < rows; r += by) {
+      const float k = (float)(full + (r < rem));
+      s += k * lds[r * t.ch + c];
+      n += k;
+    }
+    const float m = s * __builtin_amdgcn_rcpf(n);
+    #pragma unroll 4
+    for (int r = first; r < rows; r += by) {
+      const float d = lds[r * t.ch + c] - m;
+      q += lds[plane + r * t.ch + c] + (float)(full + (r < rem)) * d * d;
+    }
+    mean_o = m;
+    m2_o = q;
+    return n;
+  };
+  const int share = min(min((int)blockDim.x / t.ch, rows), 8);      // threads that share a column
+  if (share > 1) {
+    float* count = lds + 2 * plane;
+    const int s = (int)threadIdx.x / t.ch, c = (int)threadIdx.x - s * t.ch;
+    if (s < share) {
+      float m, q;
+      const float n = join(s, share, c, m, q);
+      lds[s * t.ch + c] = m;                  // row s was this thread's own
+      lds[plane + s * t.ch + c] = q;
+      if (c == 0) count[s] = n;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < t.ch) {
+      float sum = 0.0f, q = 0.0f;
+      #pragma unroll 4
+      for (int r = 0; r < share; ++r) sum += count[r] * lds[r * t.ch + c];
+      const float m = sum * inv_np;
+      #pragma unroll 4
+      for (int r = 0; r < share; ++r) {
+        const float d = lds[r * t.ch + c] - m;
+        q += lds[plane + r * t.ch + c] + count[r] * d * d;
+      }
+      out[c] = m;
+      out[t.ch + c] = q;
+    }
+  } else {
+    for (int c = threadIdx.x; c < t.ch; c += blockDim.x) join(0, 1, c, out[c], out[t.ch + c]);
+  }
+  __syncthreads();
+}
+
+// mean and sum of squares around it of a thread's own pixels, channel by channel
+template <typename T, int VEC, int R>
+__device__ __forceinline__ void own_moments(const Tile& t, const typename Pack<T, VEC>::raw (&raw)[R], int np,
+                                            float (&mean)[VEC], float (&m2)[VEC]) {
+  typedef Pack<T, VEC> P;
+  #pragma unroll
+  for (int j = 0; j < VEC; ++j) mean[j] = m2[j] = 0.0f;
+  float n = 0.0f;
+  #pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (t.on && t.r + i * t.rows < np) {
+      n += 1.0f;
+      #pragma unroll
+      for (int j = 0; j < VEC; ++j) mean[j] += P::get(raw[i], j);
+    }
+  const float inv = n > 0.0f ? 1.0f / n : 0.0f;
+  #pragma unroll
+  for (int j = 0; j < VEC; ++j) mean[j] *= inv;
+  #pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (t.on && t.r + i * t.rows < np) {
+      #pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float d = P::get(raw[i], j) - mean[j];
+        m2[j] += d * d;
+      }
+    }
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -157,8 +282,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 
 // Workgroups of one sample run one after another on one XCD, whose L2 then joins their parts of a line.
-__device__ __forceinline__ int64_t xcd_order(int64_t wg, int64_t n) {
-  const int64_t q = n / 8, rem = n % 8, xcd = wg % 8, i = wg / 8;
+__device__ __forceinline__ uint32_t xcd_order(uint32_t wg, uint32_t n) {
+  const uint32_t q = n / 8, rem = n % 8, xcd = wg % 8, i = wg / 8;
   return xcd < rem ? xcd * (q + 1) + i : rem * (q + 1) + (xcd - rem) * q + i;
 }
 
@@ -171,50 +296,28 @@ __global__ __launch_bounds__(256) void gn_chunk_stats_kernel(
     const T* __restrict__ x, float* __restrict__ ws, int S, int C, int tile, int ntile, int nchunk,
     int chunk) {
   extern __shared__ float lds[];
-  const int64_t wg = blockIdx.x;
-  const int ti = (int)(wg % ntile), ck = (int)(wg / ntile % nchunk);
-  const int64_t b = wg / ntile / nchunk;
+  const uint32_t wg = blockIdx.x, at_tile = wg / (uint32_t)ntile, at_chunk = at_tile / (uint32_t)nchunk;
+  const int ti = (int)(wg - at_tile * ntile), ck = (int)(at_tile - at_chunk * nchunk);
+  const int64_t b = at_chunk;
   const int c0 = ti * tile;
   const Tile t(min(tile, C - c0), VEC);
   const int p0 = ck * chunk, np = min(chunk, S - p0);
-  const T* xb = x + (b * S + p0) * C + c0 + t.v * VEC;
+  const T* xb = x + (b * S + p0) * C + c0;
+  const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
   typedef Pack<T, VEC> P;
   typename P::raw raw[R];
-  float acc[1][VEC];
   #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[0][j] = 0.0f;
-  #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int p = t.r + i * t.rows;
-    if (t.on && p < np) {
-      raw[i] = *(const typename P::raw*)(xb + (int64_t)p * C);
-      #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[0][j] += P::get(raw[i], j);
-    }
+  for (int i = 0; i < R; ++i)
+    if (t.on && t.r + i * t.rows < np) raw[i] = load_at<T, VEC>(xb, off + i * step);
+  float mean[VEC], m2[VEC];
+  own_moments<T, VEC, R>(t, raw, np, mean, m2);
+  float* out = lds + 2 * blockDim.x * VEC + 8;
+  channel_moments<VEC>(t, mean, m2, np, lds, out);
+  float* to = ws + (b * nchunk + ck) * 2 * C + c0;
+  for (int c = threadIdx.x; c < t.ch; c += blockDim.x) {
+    to[c] = out[c];
+    to[C + c] = out[t.ch + c];
   }
-  float* sums = lds + blockDim.x * VEC;
-  channel_sums<VEC, 1>(t, acc, lds, sums);
-  float mean[VEC];
-  #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    mean[j] = sums[t.v * VEC + j] / np;
-    acc[0][j] = 0.0f;
-  }
-  #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int p = t.r + i * t.rows;
-    if (t.on && p < np) {
-      #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = P::get(raw[i], j) - mean[j];
-        acc[0][j] += d * d;
-      }
-    }
-  }
-  float* out = ws + (b * nchunk + ck) * 2 * C + c0;
-  for (int c = threadIdx.x; c < t.ch; c += blockDim.x) out[c] = sums[c] / np;
-  channel_sums<VEC, 1>(t, acc, lds, sums);
-  for (int c = threadIdx.x; c < t.ch; c += blockDim.x) out[C + c] = sums[c];
 }
 
 // one workgroup a group: its mean, and the parts' squares moved to it
@@ -222,9 +325,9 @@ __global__ __launch_bounds__(256) void gn_join_stats_kernel(
     const float* __restrict__ ws, float* __restrict__ mean_out, float* __restrict__ rstd_out, int S,
     int C, int cg, int nchunk, int chunk, float eps) {
   __shared__ float lds[4];
-  const int G = C / cg;
-  const int64_t b = blockIdx.x / G;
-  const int g = (int)(blockIdx.x % G);
+  const uint32_t G = C / cg, bi = blockIdx.x / G;
+  const int g = (int)(blockIdx.x - bi * G);
+  const int64_t b = bi;
   const float* p = ws + b * nchunk * 2 * C + g * cg;
   float s = 0.0f;
   for (int i = threadIdx.x; i < cg * nchunk; i += blockDim.x) {
@@ -250,120 +353,184 @@ __global__ __launch_bounds__(256) void gn_join_stats_kernel(
   }
 }
 
-// what a thread needs to know of its VEC channels
-template <typename T, int VEC>
-struct Channels {
-  float mean[VEC], rstd[VEC], w[VEC], b[VEC];
-  __device__ __forceinline__ void load(const float* mean_p, const float* rstd_p, const void* wp,
-                                       const void* bp, bool f32, int c0, int cg) {
-    int g = c0 / cg, left = cg - (c0 - g * cg);
-    #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      mean[j] = mean_p[g];
-      rstd[j] = rstd_p[g];
-      w[j] = param<T>(wp, f32, c0 + j, 1.0f);
-      b[j] = param<T>(bp, f32, c0 + j, 0.0f);
-      if (--left == 0 && j + 1 < VEC) { ++g; left = cg; }
-    }
-  }
-};
+// ------------------------------------------------------------ a channel's constants
+
+// z = x a + c with a = rstd w, c = b - mean a;  xhat = x rstd + shift with shift = -mean rstd;
+// dx = dz a + x p + q with p = -rstd^2 m2, q = -rstd m1 - shift rstd m2   (m1, m2: means of u, u xhat).
+// A mean far from zero costs these the digits that it costs the mean itself; so it does to
+// sum dz xhat = rstd sum dz x + shift sum dz, which leaves the loop with two constants a channel.
+// A workgroup makes them once for its tile, in LDS; a thread then has those of its VEC channels.
+template <int VEC>
+__device__ __forceinline__ void read_vec(const float* table, int c, float (&out)[VEC]) {
+  #pragma unroll
+  for (int j = 0; j < VEC; ++j) out[j] = table[c + j];
+}
 
 template <typename T, int VEC, int R>
 __global__ __launch_bounds__(256) void gn_chunk_apply_kernel(
     const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ bias, bool f32,
     const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ y, int S, int C,
     int cg, int tile, int ntile, int nchunk, int chunk, int act) {
-  const int64_t wg = blockIdx.x;
-  const int ti = (int)(wg % ntile), ck = (int)(wg / ntile % nchunk);
-  const int64_t b = wg / ntile / nchunk;
+  extern __shared__ float lds[];                // {a, c} x tile
+  // last chunks first: they were read last, and may still be in the cache behind the L2s
+  const uint32_t wg = gridDim.x - 1 - blockIdx.x, at_tile = wg / (uint32_t)ntile, at_chunk = at_tile / (uint32_t)nchunk;
+  const int ti = (int)(wg - at_tile * ntile), ck = (int)(at_tile - at_chunk * nchunk);
+  const int64_t b = at_chunk;
   const int c0 = ti * tile;
   const Tile t(min(tile, C - c0), VEC);
-  if (!t.on) return;
   const int p0 = ck * chunk, np = min(chunk, S - p0), G = C / cg;
-  const int64_t at = (b * S + p0) * C + c0 + t.v * VEC;
+  const int64_t at = (b * S + p0) * C + c0;
+  const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
   typedef Pack<T, VEC> P;
-  Channels<T, VEC> ch;
-  ch.load(mean + b * G, rstd + b * G, w, bias, f32, c0 + t.v * VEC, cg);
+  typename P::raw raw[R];
   #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int p = t.r + i * t.rows;
-    if (p < np) {
-      typename P::raw in = *(const typename P::raw*)(x + at + (int64_t)p * C), out;
-      #pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        P::set(out, j, act_value((P::get(in, j) - ch.mean[j]) * ch.rstd[j] * ch.w[j] + ch.b[j], act));
-      *(typename P::raw*)(y + at + (int64_t)p * C) = out;
+    if (t.on && p < np) raw[i] = load_at<T, VEC>(x + at, off + i * step);
+  }
+  for (int c = threadIdx.x; c < t.ch; c += blockDim.x) {
+    const int64_t g = b * G + (c0 + c) / cg;
+    const float a = rstd[g] * param<T>(w, f32, c0 + c, 1.0f);
+    lds[c] = a;
+    lds[tile + c] = param<T>(bias, f32, c0 + c, 0.0f) - mean[g] * a;
+  }
+  __syncthreads();
+  if (!t.on) return;
+  float a[VEC], c[VEC];
+  read_vec<VEC>(lds, t.v * VEC, a);
+  read_vec<VEC>(lds + tile, t.v * VEC, c);
+  by_act(act, [&](auto A) {
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int p = t.r + i * t.rows;
+      if (p < np) {
+        typename P::raw out;
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          P::set(out, j, act_value<A.value>(P::get(raw[i], j) * a[j] + c[j]));
+        store_at<T, VEC>(y + at, off + i * step, out);
+      }
     }
+  });
+}
+
+// the constants of the backward pass's first half: {rstd, shift, a, c} x tile
+template <typename T>
+__device__ __forceinline__ void backward_table(float* table, int tile, int ch, int c0, int cg,
+                                               const float* mean, const float* rstd, const void* w,
+                                               const void* bias, bool f32) {
+  for (int c = threadIdx.x; c < ch; c += blockDim.x) {
+    const int g = (c0 + c) / cg;
+    const float r = rstd[g], shift = -mean[g] * r, wc = param<T>(w, f32, c0 + c, 1.0f);
+    table[c] = r;
+    table[tile + c] = shift;
+    table[2 * tile + c] = r * wc;
+    table[3 * tile + c] = param<T>(bias, f32, c0 + c, 0.0f) + shift * wc;
   }
 }
 
-// ws[sample][chunk][{sum dz, sum dz xhat}][C]
-template <typename T, int VEC, int R>
+// ws[sample][chunk][{sum dz, sum dz xhat}][C]. A chunk is R/H groups of H loads a thread.
+template <typename T, int VEC, int R, int H>
 __global__ __launch_bounds__(256) void gn_chunk_grads_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ w,
     const void* __restrict__ bias, bool f32, const float* __restrict__ mean,
     const float* __restrict__ rstd, float* __restrict__ ws, int S, int C, int cg, int tile, int ntile,
     int nchunk, int chunk, int act) {
   extern __shared__ float lds[];
-  const int64_t wg = blockIdx.x;
-  const int ti = (int)(wg % ntile), ck = (int)(wg / ntile % nchunk);
-  const int64_t b = wg / ntile / nchunk;
+  const uint32_t wg = blockIdx.x, at_tile = wg / (uint32_t)ntile, at_chunk = at_tile / (uint32_t)nchunk;
+  const int ti = (int)(wg - at_tile * ntile), ck = (int)(at_tile - at_chunk * nchunk);
+  const int64_t b = at_chunk;
   const int c0 = ti * tile;
   const Tile t(min(tile, C - c0), VEC);
   const int p0 = ck * chunk, np = min(chunk, S - p0), G = C / cg;
-  const int64_t at = (b * S + p0) * C + c0 + t.v * VEC;
+  const int64_t at = (b * S + p0) * C + c0;
+  const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
   typedef Pack<T, VEC> P;
+  float* table = lds + 2 * blockDim.x * VEC;
+  float* sums = table + 4 * tile;
+  backward_table<T>(table, tile, t.ch, c0, cg, mean + b * G, rstd + b * G, w, bias, f32);
+  __syncthreads();
   float acc[2][VEC];
   #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[0][j] = acc[1][j] = 0.0f;
   if (t.on) {
-    Channels<T, VEC> ch;
-    ch.load(mean + b * G, rstd + b * G, w, bias, f32, c0 + t.v * VEC, cg);
-    #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int p = t.r + i * t.rows;
-      if (p < np) {
-        typename P::raw xr = *(const typename P::raw*)(x + at + (int64_t)p * C);
-        typename P::raw dr = *(const typename P::raw*)(dy + at + (int64_t)p * C);
+    float a[VEC], c[VEC];
+    read_vec<VEC>(table + 2 * tile, t.v * VEC, a);
+    read_vec<VEC>(table + 3 * tile, t.v * VEC, c);
+    by_act(act, [&](auto A) {
+      #pragma unroll 1
+      for (int o = 0; o < R; o += H) {
+        typename P::raw xr[H], dr[H];
         #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float xh = (P::get(xr, j) - ch.mean[j]) * ch.rstd[j];
-          const float dz = P::get(dr, j) * act_slope(xh * ch.w[j] + ch.b[j], act);
-          acc[0][j] += dz;
-          acc[1][j] += dz * xh;
-        }
+        for (int i = 0; i < H; ++i)
+          if (t.r + (o + i) * t.rows < np) {
+            xr[i] = load_at<T, VEC>(x + at, off + (o + i) * step);
+            dr[i] = load_at<T, VEC>(dy + at, off + (o + i) * step);
+          }
+        #pragma unroll
+        for (int i = 0; i < H; ++i)
+          if (t.r + (o + i) * t.rows < np) {
+            #pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              const float xv = P::get(xr[i], j);
+              const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+              acc[0][j] += dz;
+              acc[1][j] += dz * xv;
+            }
+          }
       }
-    }
+    });
   }
-  float* sums = lds + 2 * blockDim.x * VEC;
   channel_sums<VEC, 2>(t, acc, lds, sums);
   float* out = ws + (b * nchunk + ck) * 2 * C + c0;
-  for (int i = threadIdx.x; i < 2 * t.ch; i += blockDim.x) {
-    const int k = i / t.ch;
-    out[(int64_t)k * C + i - k * t.ch] = sums[i];
+  for (int i = threadIdx.x; i < t.ch; i += blockDim.x) {
+    out[i] = sums[i];
+    out[C + i] = table[i] * sums[t.ch + i] + table[tile + i] * sums[i];
   }
 }
 
-// means[sample][group] = {mean u, mean u xhat}
+// one workgroup a group: means[sample][group] = {mean u, mean u xhat}, and the chunks' sums joined a channel
+// to sample[sample][{sum dz, sum dz xhat}][C], which the parameters' gradients are made of
 template <typename T>
 __global__ __launch_bounds__(256) void gn_join_grads_kernel(
-    const float* __restrict__ ws, const void* __restrict__ w, bool f32, float* __restrict__ means, int S,
-    int C, int cg, int nchunk) {
-  __shared__ float lds[4];
-  const int G = C / cg;
-  const int64_t b = blockIdx.x / G;
-  const int g = (int)(blockIdx.x % G);
+    const float* __restrict__ ws, const void* __restrict__ w, bool f32, float* __restrict__ means,
+    float* __restrict__ sample, int S, int C, int cg, int nchunk) {
+  __shared__ float lds[2][256];
+  __shared__ float red[4];
+  const uint32_t G = C / cg, bi = blockIdx.x / G;
+  const int g = (int)(blockIdx.x - bi * G);
+  const int64_t b = bi;
   const float* p = ws + b * nchunk * 2 * C + g * cg;
+  const int wide = min(cg, 256), parts = 256 / wide, part = (int)threadIdx.x / wide,
+            col = (int)threadIdx.x - part * wide;
   float s1 = 0.0f, s2 = 0.0f;
-  for (int i = threadIdx.x; i < cg * nchunk; i += blockDim.x) {
-    const int k = i / cg, c = i - k * cg;
-    const float wc = param<T>(w, f32, g * cg + c, 1.0f);
-    s1 += wc * p[(int64_t)k * 2 * C + c];
-    s2 += wc * p[(int64_t)k * 2 * C + C + c];
+  for (int c0 = 0; c0 < cg; c0 += wide) {
+    const int c = c0 + col;
+    float a = 0.0f, d = 0.0f;
+    if (part < parts && c < cg)
+      for (int k = part; k < nchunk; k += parts) {
+        a += p[(int64_t)k * 2 * C + c];
+        d += p[(int64_t)k * 2 * C + C + c];
+      }
+    __syncthreads();
+    lds[0][threadIdx.x] = a;
+    lds[1][threadIdx.x] = d;
+    __syncthreads();
+    if (part == 0 && c < cg) {
+      for (int k = 1; k < parts; ++k) {
+        a += lds[0][k * wide + col];
+        d += lds[1][k * wide + col];
+      }
+      sample[b * 2 * C + g * cg + c] = a;
+      sample[b * 2 * C + C + g * cg + c] = d;
+      const float wc = param<T>(w, f32, g * cg + c, 1.0f);
+      s1 += wc * a;
+      s2 += wc * d;
+    }
   }
-  s1 = faa_block_reduce_sum(s1, lds);
+  s1 = faa_block_reduce_sum(s1, red);
   __syncthreads();
-  s2 = faa_block_reduce_sum(s2, lds);
+  s2 = faa_block_reduce_sum(s2, red);
   if (threadIdx.x == 0) {
     const float count = (float)cg * (float)S;
     means[2 * (int64_t)blockIdx.x] = s1 / count;
@@ -371,46 +538,235 @@ __global__ __launch_bounds__(256) void gn_join_grads_kernel(
   }
 }
 
-template <typename T, int VEC, int R>
+template <typename T, int VEC, int R, int H>
 __global__ __launch_bounds__(256) void gn_chunk_dx_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ w,
     const void* __restrict__ bias, bool f32, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ means, T* __restrict__ dx, int S, int C,
     int cg, int tile, int ntile, int nchunk, int chunk, int act) {
-  const int64_t wg = blockIdx.x;
-  const int ti = (int)(wg % ntile), ck = (int)(wg / ntile % nchunk);
-  const int64_t b = wg / ntile / nchunk;
+  extern __shared__ float lds[];                // {a, c, p, q} x tile
+  // last chunks first: they were read last, and may still be in the cache behind the L2s
+  const uint32_t wg = gridDim.x - 1 - blockIdx.x, at_tile = wg / (uint32_t)ntile, at_chunk = at_tile / (uint32_t)nchunk;
+  const int ti = (int)(wg - at_tile * ntile), ck = (int)(at_tile - at_chunk * nchunk);
+  const int64_t b = at_chunk;
   const int c0 = ti * tile;
   const Tile t(min(tile, C - c0), VEC);
-  if (!t.on) return;
   const int p0 = ck * chunk, np = min(chunk, S - p0), G = C / cg;
-  const int64_t at = (b * S + p0) * C + c0 + t.v * VEC;
+  const int64_t at = (b * S + p0) * C + c0;
+  const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
   typedef Pack<T, VEC> P;
-  Channels<T, VEC> ch;
-  ch.load(mean + b * G, rstd + b * G, w, bias, f32, c0 + t.v * VEC, cg);
-  float m1[VEC], m2[VEC];
-  int g = (c0 + t.v * VEC) / cg, left = cg - (c0 + t.v * VEC - g * cg);
-  #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    m1[j] = means[2 * (b * G + g)];
-    m2[j] = means[2 * (b * G + g) + 1];
-    if (--left == 0 && j + 1 < VEC) { ++g; left = cg; }
+  for (int c = threadIdx.x; c < t.ch; c += blockDim.x) {
+    const int64_t g = b * G + (c0 + c) / cg;
+    const float r = rstd[g], shift = -mean[g] * r, wc = param<T>(w, f32, c0 + c, 1.0f);
+    const float m1 = means[2 * g], m2 = means[2 * g + 1];
+    lds[c] = r * wc;
+    lds[tile + c] = param<T>(bias, f32, c0 + c, 0.0f) + shift * wc;
+    lds[2 * tile + c] = -r * r * m2;
+    lds[3 * tile + c] = -r * (m1 + shift * m2);
   }
+  __syncthreads();
+  if (!t.on) return;
+  float a[VEC], c[VEC], pp[VEC], q[VEC];
+  read_vec<VEC>(lds, t.v * VEC, a);
+  read_vec<VEC>(lds + tile, t.v * VEC, c);
+  read_vec<VEC>(lds + 2 * tile, t.v * VEC, pp);
+  read_vec<VEC>(lds + 3 * tile, t.v * VEC, q);
+  by_act(act, [&](auto A) {
+    #pragma unroll 1
+    for (int o = 0; o < R; o += H) {
+      typename P::raw xr[H], dr[H];
+      #pragma unroll
+      for (int i = 0; i < H; ++i)
+        if (t.r + (o + i) * t.rows < np) {
+          xr[i] = load_at<T, VEC>(x + at, off + (o + i) * step);
+          dr[i] = load_at<T, VEC>(dy + at, off + (o + i) * step);
+        }
+      #pragma unroll
+      for (int i = 0; i < H; ++i)
+        if (t.r + (o + i) * t.rows < np) {
+          typename P::raw out;
+          #pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float xv = P::get(xr[i], j);
+            const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+            P::set(out, j, dz * a[j] + (xv * pp[j] + q[j]));
+          }
+          store_at<T, VEC>(dx + at, off + (o + i) * step, out);
+        }
+    }
+  });
+}
+
+// ------------------------------------------------------------ a map that stays in registers
+
+// out[g] = sum of a tile's channel sums over each of its groups, a wave a group
+__device__ __forceinline__ void group_sums(const float* sums, float* out, int ch, int cg) {
+  const int lane = threadIdx.x & 63, waves = (int)blockDim.x >> 6;
+  for (int g = (int)threadIdx.x >> 6; g < ch / cg; g += waves) {
+    float s = 0.0f;
+    for (int c = lane; c < cg; c += 64) s += sums[g * cg + c];
+    s = wave_sum(s);
+    if (lane == 0) out[g] = s;
+  }
+  __syncthreads();
+}
+
+// A workgroup takes all pixels of `tile` channels (whole groups) of one sample: x is read once.
+template <typename T, int VEC, int R>
+__global__ __launch_bounds__(1024) void gn_whole_fwd_kernel(
+    const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ bias, bool f32,
+    T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out, int S, int C, int cg,
+    int tile, int ntile, int act, float eps) {
+  extern __shared__ float lds[];
+  const uint32_t wg = xcd_order(blockIdx.x, gridDim.x), bi = wg / (uint32_t)ntile;
+  const int c0 = (int)(wg - bi * ntile) * tile;
+  const int64_t b = bi;
+  const Tile t(min(tile, C - c0), VEC);
+  const int64_t at = b * S * C + c0;
+  const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
+  float* channels = lds + 2 * blockDim.x * VEC + 8; // {mean, m2} x channels
+  float* groups = channels + 2 * tile;              // {mean, rstd} x groups
+  typedef Pack<T, VEC> P;
+  typename P::raw raw[R];
+  #pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (t.on && t.r + i * t.rows < S) raw[i] = load_at<T, VEC>(x + at, off + i * step);
+  float m[VEC], m2[VEC];
+  own_moments<T, VEC, R>(t, raw, S, m, m2);
+  channel_moments<VEC>(t, m, m2, S, lds, channels);
+  const int64_t g0 = b * (C / cg) + c0 / cg;
+  const int lane = threadIdx.x & 63;
+  for (int g = (int)threadIdx.x >> 6; g < t.ch / cg; g += (int)blockDim.x >> 6) {     // a wave a group
+    float s = 0.0f, q = 0.0f;
+    for (int c = lane; c < cg; c += 64) s += channels[g * cg + c];
+    const float mean = wave_sum(s) / (float)cg;
+    for (int c = lane; c < cg; c += 64) {
+      const float d = channels[g * cg + c] - mean;
+      q += channels[t.ch + g * cg + c] + (float)S * d * d;
+    }
+    const float rstd = 1.0f / sqrtf(wave_sum(q) / ((float)cg * (float)S) + eps);
+    if (lane == 0) {
+      groups[2 * g] = mean;
+      groups[2 * g + 1] = rstd;
+      mean_out[g0 + g] = mean;
+      rstd_out[g0 + g] = rstd;
+    }
+  }
+  __syncthreads();
+  // a and c of every channel take the place of the rows
+  for (int c = threadIdx.x; c < t.ch; c += blockDim.x) {
+    const int g = c / cg;
+    const float a = groups[2 * g + 1] * param<T>(w, f32, c0 + c, 1.0f);
+    lds[c] = a;
+    lds[tile + c] = param<T>(bias, f32, c0 + c, 0.0f) - groups[2 * g] * a;
+  }
+  __syncthreads();
+  if (!t.on) return;
+  float a[VEC], c[VEC];
+  read_vec<VEC>(lds, t.v * VEC, a);
+  read_vec<VEC>(lds + tile, t.v * VEC, c);
+  by_act(act, [&](auto A) {
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int p = t.r + i * t.rows;
+      if (p < S) {
+        typename P::raw out;
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          P::set(out, j, act_value<A.value>(P::get(raw[i], j) * a[j] + c[j]));
+        store_at<T, VEC>(y + at, off + i * step, out);
+      }
+    }
+  });
+}
+
+// x and dy are read once; sample[b][{sum dz, sum dz xhat}][C] goes to the parameters' gradients
+template <typename T, int VEC, int R>
+__global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ w,
+    const void* __restrict__ bias, bool f32, const float* __restrict__ mean_in,
+    const float* __restrict__ rstd_in, T* __restrict__ dx, float* __restrict__ sample, int S, int C, int cg,
+    int tile, int ntile, int act) {
+  extern __shared__ float lds[];
+  const uint32_t wg = xcd_order(blockIdx.x, gridDim.x), bi = wg / (uint32_t)ntile;
+  const int c0 = (int)(wg - bi * ntile) * tile;
+  const int64_t b = bi;
+  const Tile t(min(tile, C - c0), VEC);
+  const int64_t at = b * S * C + c0, g0 = b * (C / cg);
+  const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
+  float* table = lds + 2 * blockDim.x * VEC;    // {rstd, shift, a, c} x tile
+  float* sums = table + 4 * tile;               // {dz, dz xhat} x channels
+  float* groups = sums + 2 * tile;              // {u, u xhat} x groups
+  typedef Pack<T, VEC> P;
+  typename P::raw xr[R], dr[R];
   #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int p = t.r + i * t.rows;
-    if (p < np) {
-      typename P::raw xr = *(const typename P::raw*)(x + at + (int64_t)p * C);
-      typename P::raw dr = *(const typename P::raw*)(dy + at + (int64_t)p * C), out;
-      #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float xh = (P::get(xr, j) - ch.mean[j]) * ch.rstd[j];
-        const float dz = P::get(dr, j) * act_slope(xh * ch.w[j] + ch.b[j], act);
-        P::set(out, j, ch.rstd[j] * (dz * ch.w[j] - m1[j] - xh * m2[j]));
-      }
-      *(typename P::raw*)(dx + at + (int64_t)p * C) = out;
+    if (t.on && p < S) {
+      xr[i] = load_at<T, VEC>(x + at, off + i * step);
+      dr[i] = load_at<T, VEC>(dy + at, off + i * step);
     }
   }
+  backward_table<T>(table, tile, t.ch, c0, cg, mean_in + g0, rstd_in + g0, w, bias, f32);
+  __syncthreads();
+  float a[VEC], c[VEC];
+  read_vec<VEC>(table + 2 * tile, t.v * VEC, a);
+  read_vec<VEC>(table + 3 * tile, t.v * VEC, c);
+  float acc[2][VEC];
+  #pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[0][j] = acc[1][j] = 0.0f;
+  by_act(act, [&](auto A) {
+    #pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (t.on && t.r + i * t.rows < S) {
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float xv = P::get(xr[i], j);
+          const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+          acc[0][j] += dz;
+          acc[1][j] += dz * xv;
+        }
+      }
+  });
+  channel_sums<VEC, 2>(t, acc, lds, sums);
+  for (int i = threadIdx.x; i < t.ch; i += blockDim.x) {
+    const float s1 = sums[i], s2 = table[i] * sums[t.ch + i] + table[tile + i] * s1;
+    const float wc = param<T>(w, f32, c0 + i, 1.0f);
+    sample[b * 2 * C + c0 + i] = s1;
+    sample[(b * 2 + 1) * C + c0 + i] = s2;
+    sums[i] = s1 * wc;
+    sums[t.ch + i] = s2 * wc;
+  }
+  __syncthreads();
+  group_sums(sums, groups, 2 * t.ch, cg);       // both planes: a tile is whole groups
+  const float inv = 1.0f / ((float)cg * (float)S);
+  for (int i = threadIdx.x; i < t.ch; i += blockDim.x) {
+    const int g = i / cg;
+    const float m1 = groups[g] * inv, m2 = groups[t.ch / cg + g] * inv, r = table[i], shift = table[tile + i];
+    table[i] = -r * r * m2;
+    table[tile + i] = -r * (m1 + shift * m2);
+  }
+  __syncthreads();
+  if (!t.on) return;
+  float pp[VEC], q[VEC];
+  read_vec<VEC>(table, t.v * VEC, pp);
+  read_vec<VEC>(table + tile, t.v * VEC, q);
+  by_act(act, [&](auto A) {
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int p = t.r + i * t.rows;
+      if (p < S) {
+        typename P::raw out;
+        #pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float xv = P::get(xr[i], j);
+          const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+          P::set(out, j, dz * a[j] + (xv * pp[j] + q[j]));
+        }
+        store_at<T, VEC>(dx + at, off + i * step, out);
+      }
+    }
+  });
 }
 
 // dw[c], db[c]: the sums over n rows of ws[row][{sum dz, sum dz xhat}][C], 32 columns a workgroup
@@ -441,33 +797,43 @@ __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const float* __res
 struct Shape {
   int64_t B;
   int S, C, G, cg;
-  bool vec;
 };
 
-Shape shape_of(const torch::Tensor& x, int64_t groups) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.dim() == 3, "group_norm: [N, pixels, C] expected");
+// x: [N, ..., C], contiguous
+Shape shape_of(const torch::Tensor& x, int64_t groups, const torch::Tensor& w, const torch::Tensor& b,
+               int64_t act) {
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.dim() >= 2, "group_norm_act: [N, C, ...] on the GPU");
   Shape s;
   s.B = x.size(0);
-  TORCH_CHECK(x.size(1) * x.size(2) < (int64_t(1) << 31), "group_norm: a sample has 2^31 values or more");
-  s.S = (int)x.size(1);
-  s.C = (int)x.size(2);
-  TORCH_CHECK(groups > 0 && s.C % groups == 0, "group_norm: C is no multiple of the groups");
+  const int64_t C = x.size(-1), S = x.numel() ? x.numel() / (s.B * C) : 0;
+  TORCH_CHECK(S * C < (int64_t(1) << 31), "group_norm_act: a sample has 2^31 values or more");
+  TORCH_CHECK(C < (1 << 23), "group_norm_act: 2^23 channels or more");
+  TORCH_CHECK(groups > 0 && C > 0 && C % groups == 0, "group_norm_act: C is no multiple of the groups");
+  s.S = (int)S;
+  s.C = (int)C;
   s.G = (int)groups;
   s.cg = s.C / s.G;
+  for (const auto* p : {&w, &b})
+    TORCH_CHECK(!p->defined() || (p->is_contiguous() && p->dim() == 1 && p->size(0) == C
+                && p->device() == x.device()
+                && (p->scalar_type() == x.scalar_type() || p->scalar_type() == torch::kFloat32)),
+                "group_norm_act: weight and bias are [C], of the map's type or fp32");
+  TORCH_CHECK(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
+              "group_norm_act: weight and bias are of one type");
+  TORCH_CHECK(act >= 0 && act <= 2, "group_norm_act: activation");
   return s;
+}
+
+const void* data(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+bool is_f32(const torch::Tensor& w, const torch::Tensor& b) {
+  return (w.defined() && w.scalar_type() == torch::kFloat32)
+         || (b.defined() && b.scalar_type() == torch::kFloat32);
 }
 
 bool aligned16(std::initializer_list<const torch::Tensor*> ts) {
   for (auto* t : ts)
     if (reinterpret_cast<uintptr_t>(t->data_ptr()) % 16) return false;
   return true;
-}
-
-void check_param(const c10::optional<torch::Tensor>& p, const torch::Tensor& x, int C) {
-  if (!p.has_value()) return;
-  TORCH_CHECK(p->is_contiguous() && p->dim() == 1 && p->size(0) == C && p->device() == x.device()
-              && (p->scalar_type() == x.scalar_type() || p->scalar_type() == torch::kFloat32),
-              "group_norm: weight and bias are [C], of the map's type or fp32");
 }
 
 // chunks of pixels and tiles of channels for workgroups of 256
@@ -493,116 +859,227 @@ void by_type(torch::ScalarType t, F f) {
   else TORCH_CHECK(false, "group_norm: fp32, bf16 and fp16 are taken");
 }
 
-constexpr int kR = 8;
+// How a map is cut where its pixels fit the registers of a workgroup.
+struct Whole { int tile, ntile, threads, r; };
+
+// Tiles are whole groups and whole vectors. About 2048 vectors of 16 bytes a workgroup are aimed at (256 threads
+// with 8 each: several workgroups fit a CU, and some load while others add up): wide tiles where the map is
+// small, down to lines of 128, 64 and 32 bytes as long as there are fewer than 1024, 512 and 256 workgroups.
+// Over 4096 vectors a CU holds one workgroup or two and waits for each of its phases, and the chunks' second
+// read is cheaper, unless all workgroups run at once, when lines of 32 bytes do too. Measured (bf16, forward +
+// backward, us, whole/chunks): 128x14x14x1024 26+40/41+64, 128x28x28x512 41+98/62+104, 128x56x56x64 26+53/40+62,
+// 128x56x56x256 136+263/125+211.
+template <typename T, int VEC, int MOST_R>
+bool whole_of(const Shape& s, Whole& out) {
+  const int64_t unit = std::lcm((int64_t)s.cg, (int64_t)VEC), line = sizeof(T) * unit;
+  if ((int64_t)s.S * s.C * sizeof(T) >= (int64_t(1) << 30) || unit / VEC > 256) return false;   // offsets: 32 bits
+  const int64_t units = s.C / unit, sixteen = 16 / sizeof(T);
+  auto vectors = [&](int64_t k) { return k * unit * s.S / sixteen; };
+  auto workgroups = [&](int64_t k) { return s.B * ((units + k - 1) / k); };
+  auto lines = [&](int64_t bytes) { return std::min(units, std::max<int64_t>(1, bytes / line)); };
+  int64_t k = std::min(units, std::max(lines(64), 2048 / std::max<int64_t>(1, vectors(1))));
+  for (int bytes : {128, 64, 32})
+    while (k > lines(bytes) && workgroups(k) < 8 * bytes) k = std::max(lines(bytes), k / 2);
+  if (vectors(k) > 4096) {
+    k = lines(32);
+    if (vectors(k) > 8192 || workgroups(k) < 256 || workgroups(k) > 768) return false;
+  }
+  out.tile = (int)(k * unit);
+  out.ntile = (int)((units + k - 1) / k);
+  if (workgroups(k) >= (int64_t(1) << 31)) return false;
+  for (int threads : {256, 512, 1024})
+    for (out.r = 1; out.r <= MOST_R; out.r *= 2) {
+      out.threads = (int)((((int64_t)s.S + out.r - 1) / out.r * (out.tile / VEC) + 63) / 64 * 64);
+      if (out.threads <= threads) return true;
+    }
+  return false;
+}
+
+// f(r as a constant), r a power of 2 up to MOST
+template <int MOST, typename F>
+void by_r(int r, F f) {
+  if constexpr (MOST > 1) {
+    if (r < MOST) return by_r<MOST / 2>(r, f);
+  }
+  f(std::integral_constant<int, MOST>{});
+}
+// f(values a load): 16 bytes, or 8 where 16 do not divide a line of channels, or where whole groups of whole
+// 16 bytes are too much for a workgroup and those of 8 are less (EfficientNet's 84 channels a group: 20+39 us
+// with 16 bytes, see 100x14x14x672)
+template <typename T, typename F>
+void by_vec(const Shape& s, bool aligned, F f) {
+  constexpr int V = 16 / sizeof(T);
+  if constexpr (V == 8) {
+    const int64_t u8 = std::lcm((int64_t)s.cg, (int64_t)8), u4 = std::lcm((int64_t)s.cg, (int64_t)4);
+    if (aligned && s.C % 4 == 0 && (s.C % 8 != 0 || (u4 < u8 && u8 * s.S > 2048 * 8)))
+      return f(std::integral_constant<int, 4>{});
+  }
+  if (aligned && s.C % V == 0) f(std::integral_constant<int, V>{});
+  else f(std::integral_constant<int, 1>{});
+}
+
+// vectors a thread: as many as registers hold without spilling
+template <typename T, int VEC> constexpr int kForwardR = VEC == 1 ? 32 : 16;
+template <typename T, int VEC> constexpr int kBackwardR = VEC == 1 ? 32 : (VEC * sizeof(T) == 8 ? 16 : 8);
+
+constexpr int kR = 8;       // vectors a thread in a chunk
 
 template <typename T, int VEC>
-void forward(const Shape& s, const torch::Tensor& x, const void* w, const void* b, bool f32,
+void forward_on(const Shape& s, const torch::Tensor& x, const void* w, const void* b, bool f32,
              torch::Tensor& y, torch::Tensor& mean, torch::Tensor& rstd, double eps, int act,
              hipStream_t stream) {
+  Whole p;
+  if (whole_of<T, VEC, kForwardR<T, VEC>>(s, p)) {
+    const size_t lds = (2 * (size_t)p.threads * VEC + 8 + 4 * p.tile) * sizeof(float);
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)(s.B * p.ntile)), dim3(p.threads), lds, stream,
+                         (const T*)x.data_ptr(), w, b, f32, (T*)y.data_ptr(), mean.data_ptr<float>(),
+                         rstd.data_ptr<float>(), s.S, s.C, s.cg, p.tile, p.ntile, act, (float)eps);
+    };
+    by_r<kForwardR<T, VEC>>(p.r, [&](auto r) { go(gn_whole_fwd_kernel<T, VEC, r.value>); });
+    return;
+  }
   const Chunks c = chunks_of<VEC>(s, kR);
   auto ws = torch::empty({s.B * c.nchunk * 2 * s.C}, mean.options());
-  const size_t lds = (256 * VEC + c.tile) * sizeof(float);
+  const size_t lds = (2 * 256 * VEC + 8 + 2 * c.tile) * sizeof(float);
   hipLaunchKernelGGL((gn_chunk_stats_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256), lds, stream,
                      (const T*)x.data_ptr(), ws.data_ptr<float>(), s.S, s.C, c.tile, c.ntile, c.nchunk,
                      c.chunk);
   hipLaunchKernelGGL(gn_join_stats_kernel, dim3((unsigned)(s.B * s.G)), dim3(256), 0, stream,
                      ws.data_ptr<float>(), mean.data_ptr<float>(), rstd.data_ptr<float>(), s.S, s.C,
                      s.cg, c.nchunk, c.chunk, (float)eps);
-  hipLaunchKernelGGL((gn_chunk_apply_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256), 0, stream,
-                     (const T*)x.data_ptr(), w, b, f32, mean.data_ptr<float>(), rstd.data_ptr<float>(),
+  hipLaunchKernelGGL((gn_chunk_apply_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256),
+                     2 * c.tile * sizeof(float), stream, (const T*)x.data_ptr(), w, b, f32, mean.data_ptr<float>(), rstd.data_ptr<float>(),
                      (T*)y.data_ptr(), s.S, s.C, s.cg, c.tile, c.ntile, c.nchunk, c.chunk, act);
 }
 
-// returns the rows of sums that the parameters' gradients are made of
+// returns the samples' sums, which the parameters' gradients are made of
 template <typename T, int VEC>
-torch::Tensor backward(const Shape& s, const torch::Tensor& dy, const torch::Tensor& x, const void* w,
+torch::Tensor backward_on(const Shape& s, const torch::Tensor& dy, const torch::Tensor& x, const void* w,
                        const void* b, bool f32, const torch::Tensor& mean, const torch::Tensor& rstd,
                        torch::Tensor& dx, int act, hipStream_t stream) {
+  auto sample = torch::empty({s.B, 2 * (int64_t)s.C}, mean.options());
+  Whole p;
+  if (whole_of<T, VEC, kBackwardR<T, VEC>>(s, p)) {
+    const size_t lds = (2 * (size_t)p.threads * VEC + 8 * p.tile) * sizeof(float);
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)(s.B * p.ntile)), dim3(p.threads), lds, stream,
+                         (const T*)dy.data_ptr(), (const T*)x.data_ptr(), w, b, f32,
+                         mean.data_ptr<float>(), rstd.data_ptr<float>(), (T*)dx.data_ptr(),
+                         sample.data_ptr<float>(), s.S, s.C, s.cg, p.tile, p.ntile, act);
+    };
+    by_r<kBackwardR<T, VEC>>(p.r, [&](auto r) { go(gn_whole_bwd_kernel<T, VEC, r.value>); });
+    return sample;
+  }
   const Chunks c = chunks_of<VEC>(s, kR);
   auto ws = torch::empty({s.B * c.nchunk, 2 * (int64_t)s.C}, mean.options());
   auto means = torch::empty({s.B * s.G * 2}, mean.options());
-  const size_t lds = (2 * 256 * VEC + 2 * c.tile) * sizeof(float);
-  hipLaunchKernelGGL((gn_chunk_grads_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256), lds, stream,
+  const size_t lds = (2 * 256 * VEC + 6 * c.tile) * sizeof(float);
+  hipLaunchKernelGGL((gn_chunk_grads_kernel<T, VEC, kR, 4>), dim3((unsigned)c.wgs), dim3(256), lds, stream,
                      (const T*)dy.data_ptr(), (const T*)x.data_ptr(), w, b, f32,
                      mean.data_ptr<float>(), rstd.data_ptr<float>(), ws.data_ptr<float>(), s.S, s.C,
                      s.cg, c.tile, c.ntile, c.nchunk, c.chunk, act);
   hipLaunchKernelGGL((gn_join_grads_kernel<T>), dim3((unsigned)(s.B * s.G)), dim3(256), 0, stream,
-                     ws.data_ptr<float>(), w, f32, means.data_ptr<float>(), s.S, s.C, s.cg, c.nchunk);
-  hipLaunchKernelGGL((gn_chunk_dx_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256), 0, stream,
+                     ws.data_ptr<float>(), w, f32, means.data_ptr<float>(), sample.data_ptr<float>(), s.S,
+                     s.C, s.cg, c.nchunk);
+  hipLaunchKernelGGL((gn_chunk_dx_kernel<T, VEC, kR, 4>), dim3((unsigned)c.wgs), dim3(256),
+                     4 * c.tile * sizeof(float), stream,
                      (const T*)dy.data_ptr(), (const T*)x.data_ptr(), w, b, f32,
                      mean.data_ptr<float>(), rstd.data_ptr<float>(), means.data_ptr<float>(),
                      (T*)dx.data_ptr(), s.S, s.C, s.cg, c.tile, c.ntile, c.nchunk, c.chunk, act);
-  return ws;
+  return sample;
 }
+
+class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
+ public:
+  // x: [N, C, ...] of any order
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor x, int64_t groups,
+                               c10::optional<torch::Tensor> weight, c10::optional<torch::Tensor> bias,
+                               double eps, int64_t act) {
+    const c10::OptionalDeviceGuard guard(x.device());
+    auto rows = x.movedim(1, -1).contiguous();
+    auto w = weight ? weight->contiguous() : torch::Tensor(), b = bias ? bias->contiguous() : torch::Tensor();
+    const Shape s = shape_of(rows, groups, w, b, act);
+    auto y = at::empty_strided(x.sizes(), rows.movedim(-1, 1).strides(), x.options());
+    auto stat = x.options().dtype(torch::kFloat32);
+    auto mean = torch::empty({s.B, s.G}, stat), rstd = torch::empty({s.B, s.G}, stat);
+    if (x.numel() > 0) {
+      auto stream = at::hip::getCurrentHIPStream().stream();
+      by_type(x.scalar_type(), [&](auto z) {
+        using T = decltype(z);
+        by_vec<T>(s, aligned16({&rows, &y}), [&](auto v) {
+          forward_on<T, v.value>(s, rows, data(w), data(b), is_f32(w, b), y, mean, rstd, eps, (int)act, stream);
+        });
+      });
+    }
+    C10_HIP_KERNEL_LAUNCH_CHECK();
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->save_for_backward({rows, w, b, mean, rstd});
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const bool again = at::GradMode::is_enabled();
+    auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &w = saved[1], &b = saved[2], &mean = saved[3], &rstd = saved[4];
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const c10::OptionalDeviceGuard guard(x.device());
+    auto stream = at::hip::getCurrentHIPStream().stream();
+    // absent tensors are not counted among the inputs
+    const bool nw = w.defined() && ctx->needs_input_grad(1),
+               nb = b.defined() && ctx->needs_input_grad(w.defined() ? 2 : 1);
+    torch::Tensor dx, dw, db;
+    {
+      at::NoGradGuard off;
+      const Shape s = shape_of(x, ctx->saved_data["groups"].toInt(), w, b, act);
+      auto dy = grads[0].movedim(1, -1).contiguous();
+      dx = torch::empty_like(x);
+      auto popt = (w.defined() ? w : b.defined() ? b : mean).options();
+      if (nw || nb) {
+        dw = torch::empty({s.C}, popt);
+        db = torch::empty({s.C}, popt);
+      }
+      if (x.numel() == 0) {
+        if (nw || nb) {
+          dw.zero_();
+          db.zero_();
+        }
+      } else {
+        torch::Tensor sums;
+        by_type(x.scalar_type(), [&](auto z) {
+          using T = decltype(z);
+          by_vec<T>(s, aligned16({&x, &dy, &dx}), [&](auto v) {
+            sums = backward_on<T, v.value>(s, dy, x, data(w), data(b), is_f32(w, b), mean, rstd, dx, act, stream);
+          });
+        });
+        if (nw || nb)
+          by_type(dw.scalar_type(), [&](auto z) {
+            using W = decltype(z);
+            hipLaunchKernelGGL((gn_param_grads_kernel<W>), dim3((2 * s.C + 31) / 32), dim3(1024), 0, stream,
+                               sums.data_ptr<float>(), sums.size(0), s.C, (W*)dw.data_ptr(),
+                               (W*)db.data_ptr());
+          });
+        C10_HIP_KERNEL_LAUNCH_CHECK();
+      }
+    }
+    torch::autograd::variable_list out{dx.movedim(-1, 1), torch::Tensor(), nw ? dw : torch::Tensor(),
+                                       nb ? db : torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    if (again)      // differentiating these again is an error, not a zero
+      for (auto& g : out)
+        if (g.defined()) {
+          auto err = std::make_shared<torch::autograd::DelayedError>(
+              "group_norm_act is differentiable once", 1);
+          g = (*err)({g.detach().requires_grad_(true)})[0];
+        }
+    return out;
+  }
+};
 
 }  // namespace
 
-// x: [N, pixels, C] contiguous. Returns y, mean[N, G], rstd[N, G].
-std::vector<torch::Tensor> group_norm_fwd(torch::Tensor x, int64_t groups,
-                                          c10::optional<torch::Tensor> weight,
-                                          c10::optional<torch::Tensor> bias, double eps, int64_t act) {
-  Shape s = shape_of(x, groups);
-  check_param(weight, x, s.C);
-  check_param(bias, x, s.C);
-  TORCH_CHECK(!weight || !bias || weight->scalar_type() == bias->scalar_type(),
-              "group_norm: weight and bias are of one type");
-  TORCH_CHECK(act >= 0 && act <= 2, "group_norm: activation");
-  const c10::OptionalDeviceGuard guard(x.device());
-  auto stream = at::hip::getCurrentHIPStream().stream();
-  auto y = torch::empty_like(x);
-  auto stat = x.options().dtype(torch::kFloat32);
-  auto mean = torch::empty({s.B, s.G}, stat), rstd = torch::empty({s.B, s.G}, stat);
-  if (x.numel() == 0) return {y, mean, rstd};
-  const void* w = weight ? weight->data_ptr() : nullptr;
-  const void* b = bias ? bias->data_ptr() : nullptr;
-  const auto& any = weight ? weight : bias;
-  const bool f32 = any && any->scalar_type() == torch::kFloat32;
-  by_type(x.scalar_type(), [&](auto z) {
-    using T = decltype(z);
-    constexpr int V = 16 / sizeof(T);
-    if (s.C % V == 0 && aligned16({&x, &y}))
-      forward<T, V>(s, x, w, b, f32, y, mean, rstd, eps, (int)act, stream);
-    else
-      forward<T, 1>(s, x, w, b, f32, y, mean, rstd, eps, (int)act, stream);
-  });
-  return {y, mean, rstd};
-}
-
-// Returns dx, and dweight and dbias in the parameters' type where param_grads is set.
-std::vector<torch::Tensor> group_norm_bwd(torch::Tensor dy, torch::Tensor x, int64_t groups,
-                                          c10::optional<torch::Tensor> weight,
-                                          c10::optional<torch::Tensor> bias, torch::Tensor mean,
-                                          torch::Tensor rstd, int64_t act, bool param_grads) {
-  Shape s = shape_of(x, groups);
-  check_param(weight, x, s.C);
-  check_param(bias, x, s.C);
-  TORCH_CHECK(dy.is_contiguous() && dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type()
-              && dy.device() == x.device(), "group_norm: dy is like x");
-  TORCH_CHECK(mean.numel() == s.B * s.G && rstd.numel() == mean.numel(), "group_norm: statistics");
-  const c10::OptionalDeviceGuard guard(x.device());
-  auto stream = at::hip::getCurrentHIPStream().stream();
-  auto dx = torch::empty_like(x);
-  const void* w = weight ? weight->data_ptr() : nullptr;
-  const void* b = bias ? bias->data_ptr() : nullptr;
-  const auto& any = weight ? weight : bias;
-  const bool f32 = any && any->scalar_type() == torch::kFloat32;
-  auto popt = any ? any->options() : x.options().dtype(torch::kFloat32);
-  if (x.numel() == 0) return {dx, torch::zeros({s.C}, popt), torch::zeros({s.C}, popt)};
-  torch::Tensor ws;
-  by_type(x.scalar_type(), [&](auto z) {
-    using T = decltype(z);
-    constexpr int V = 16 / sizeof(T);
-    if (s.C % V == 0 && aligned16({&x, &dy, &dx}))
-      ws = backward<T, V>(s, dy, x, w, b, f32, mean, rstd, dx, (int)act, stream);
-    else
-      ws = backward<T, 1>(s, dy, x, w, b, f32, mean, rstd, dx, (int)act, stream);
-  });
-  if (!param_grads) return {dx};
-  auto dw = torch::empty({s.C}, popt), db = torch::empty({s.C}, popt);
-  by_type(dw.scalar_type(), [&](auto z) {
-    using W = decltype(z);
-    hipLaunchKernelGGL((gn_param_grads_kernel<W>), dim3((2 * s.C + 31) / 32), dim3(1024), 0, stream,
-                       ws.data_ptr<float>(), ws.size(0), s.C, (W*)dw.data_ptr(), (W*)db.data_ptr());
-  });
-  return {dx, dw, db};
+torch::Tensor group_norm_act(torch::Tensor x, int64_t groups, c10::optional<torch::Tensor> weight,
+                             c10::optional<torch::Tensor> bias, double eps, int64_t act) {
+  return GroupNormAct::apply(x, groups, weight, bias, eps, act);
 }

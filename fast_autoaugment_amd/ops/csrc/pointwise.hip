@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
 #include <hip/hip_fp16.h>
 #include "faa_common.h"
 
@@ -634,6 +635,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
                         keep ? (T*)z.data_ptr() : nullptr, (int)act, false};
         product<T, false, false>(x, w, epi, stream);
       });
+    C10_HIP_KERNEL_LAUNCH_CHECK();
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = b.defined();
     ctx->saved_data["res"] = r.defined();
@@ -682,6 +684,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
             product<T, true, true>(dz, x, epi, stream);
           }
         });
+        C10_HIP_KERNEL_LAUNCH_CHECK();
       }
     }
     torch::autograd::variable_list out{dx, dw, db, nr ? dz : torch::Tensor(), torch::Tensor(),

@@ -10,35 +10,11 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import require_ext_for
 
 ACTS = {"none": 0, "relu": 1, "swish": 2}
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-class GroupNormActFn(torch.autograd.Function):
-    """x: [N, pixels, C], contiguous."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act):
-        C = require_ext_for(x)
-        y, mean, rstd = C.group_norm_fwd(x, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.groups, ctx.act = groups, act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        C = require_ext_for(x)
-        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
-        dx, *grads = C.group_norm_bwd(dy.contiguous(), x, ctx.groups, weight, bias, mean, rstd,
-                                      ctx.act, need_w or need_b)
-        dw, db = grads if grads else (None, None)
-        return dx, dw if need_w else None, db if need_b else None, None, None, None
 
 
 def _check(x, num_groups, weight, bias, eps, act):
@@ -97,8 +73,4 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     _check(x, num_groups, weight, bias, eps, act)
     if not x.is_cuda:
         return _composed(x, num_groups, weight, bias, eps, act)
-    rows = x.movedim(1, -1)
-    flat = rows.reshape(x.size(0), -1, x.size(1)) if x.numel() else rows.reshape(x.size(0), 0, x.size(1))
-    y = GroupNormActFn.apply(flat.contiguous(), None if weight is None else weight.contiguous(),
-                             None if bias is None else bias.contiguous(), num_groups, eps, ACTS[act])
-    return y.view(rows.shape).movedim(-1, 1)
+    return require_ext_for(x).group_norm_act(x, num_groups, weight, bias, eps, ACTS[act])
