@@ -6,16 +6,20 @@
 // One kernel computes D[m][n] = sum_k P(m,k) Q(n,k) for 16-bit types, where each
 // operand lies either with k contiguous (x and W forward) or with its rows
 // contiguous (W for dx; dz and x for dW): no transposed copy is made. A
-// workgroup of 4 waves owns a BM x BN tile, steps through k by 64, and has the
-// next step's loads in flight in registers while it multiplies out of LDS.
-// Operands with contiguous rows are turned on their way out of LDS
-// (ds_read_b64_tr_b16). The roles in the matrix instruction are swapped (its
-// rows are n), so that a lane ends with 4 neighbouring columns of one output
-// row: 8-byte loads of the residual and stores of the result.
+// workgroup of 4 waves owns a BM x BN tile and steps through k by 64; the next
+// step's pieces go from memory to LDS by themselves (buffer loads that write
+// LDS, zero outside the operand) while this one's are multiplied. Operands with
+// contiguous rows are turned on their way out of LDS (ds_read_b64_tr_b16). The
+// roles in the matrix instruction are swapped (its rows are n) and its rows are
+// dealt to n so that a lane ends with 8 neighbouring columns of an output row:
+// 16-byte loads of the residual and stores of the result.
 //
 // A long k with few output tiles (dW: k is the batch's pixels) is split over
 // workgroups; parts go to a workspace in fp32 and are added in a fixed order by
 // a second kernel, which also has the epilogue.
+//
+// Operands whose lines do not start at 16 bytes are first copied into lines
+// that do, which costs less than loads of 2 bytes in the product.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -23,6 +27,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <hip/hip_fp16.h>
+#include <type_traits>
 #include "faa_common.h"
 
 namespace {
@@ -107,22 +112,43 @@ __device__ __forceinline__ void store4(T* p, int left, bool vec, f32x4 v) {
     if (i < left) Num<T>::put(p + i, v[i]);
 }
 
+// exp2 without the range handling of expf: what it would give below 2^-126 is nothing next to 1
 __device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
-__device__ __forceinline__ float act_value(float z, int act) {
-  if (act == ACT_RELU) return z < 0.0f ? 0.0f : z;      // a NaN stays one
-  if (act == ACT_SWISH) return z * sigmoid(z);
-  if (act == ACT_SIGMOID) return sigmoid(z);
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+  if (ACT == ACT_RELU) return z < 0.0f ? 0.0f : z;      // a NaN stays one
+  if (ACT == ACT_SWISH) return z * sigmoid(z);
+  if (ACT == ACT_SIGMOID) return sigmoid(z);
   return z;
 }
 // from z, or for relu from y: both are above 0 in the same places
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   const float s = sigmoid(z);
-  if (act == ACT_SWISH) return s * (1.0f + z * (1.0f - s));
-  if (act == ACT_SIGMOID) return s * (1.0f - s);
+  if (ACT == ACT_SWISH) return s + s * (z - z * s);
+  if (ACT == ACT_SIGMOID) return s - s * s;
   return 1.0f;
+}
+// f(activation as a constant): one branch outside the loops, not one an element
+template <typename F>
+__device__ __forceinline__ void by_act(int act, F f) {
+  if (act == ACT_SWISH) f(std::integral_constant<int, ACT_SWISH>{});
+  else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  else if (act == ACT_SIGMOID) f(std::integral_constant<int, ACT_SIGMOID>{});
+  else f(std::integral_constant<int, ACT_NONE>{});
+}
+
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+
+template <typename T>
+__device__ __forceinline__ f32x8 widen8(s16x8 u) {
+  f32x8 v;
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = Num<T>::of(u[i]);
+  return v;
 }
 
 // ------------------------------------------------------------ epilogue
@@ -134,135 +160,163 @@ struct Epilogue {
   T* y;               // [M,N]
   T* z;               // [M,N] or null: the sum before the activation, for the backward pass
   int act;
-  bool vec;           // rows of 4 may be read and written at once
+  bool vec;           // rows of 4 (8 in 16 bits) may be read and written at once
 
-  __device__ __forceinline__ void operator()(int64_t m, int n, int N, f32x4 v) const {
+  // 4 columns from n of row m
+  template <int ACT>
+  __device__ __forceinline__ void four(int64_t m, int n, int N, f32x4 v) const {
     const int left = N - n;
     if (left <= 0) return;
     const int64_t at = m * N + n;
     if (bias) v += load4(bias + n, left, vec);
     if (res) v += load4(res + at, left, vec);
-    if (z) {
-      store4(z + at, left, vec, v);
-      // the backward pass has z in its own type; y is that of the exact sum
-    }
-    if (act != ACT_NONE) {
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = act_value(v[i], act);
-    }
+    if (z) store4(z + at, left, vec, v);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(v[i]);
     store4(y + at, left, vec, v);
+  }
+  // 8 columns, 16 bytes at once
+  template <int ACT>
+  __device__ __forceinline__ void eight(int64_t at, f32x8 v, f32x8 b) const {
+    v += b;
+    if (res) v += widen8<T>(*(const s16x8*)(res + at));
+    s16x8 out;
+    if (z) {
+      #pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = Num<T>::bits(v[e]);
+      *(s16x8*)(z + at) = out;
+    }
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) out[e] = Num<T>::bits(act_value<ACT>(v[e]));
+    *(s16x8*)(y + at) = out;
   }
 };
 
 // ------------------------------------------------------------ operands
 
-// P(row, k): row-major with k contiguous, or (ROWS) k-major with rows contiguous
-template <typename T>
+// P(row, k): row-major with k contiguous, or (ROWS) k-major with rows contiguous. Lines start at 16 bytes.
 struct Operand {
-  const T* p;
+  const short* p;
   int rows, kdim;
-  int64_t ld;
-  bool vec;           // 8 neighbours may be loaded at once, and none of them lies over the edge
+  int64_t ld;         // a multiple of 8
 };
 
-template <typename T, bool ROWS>
-__device__ __forceinline__ s16x8 load8(const Operand<T>& o, int row, int k) {
-  s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (ROWS ? k >= o.kdim : row >= o.rows) return v;
-  const T* p = ROWS ? o.p + (int64_t)k * o.ld + row : o.p + (int64_t)row * o.ld + k;
-  const int left = ROWS ? o.rows - row : o.kdim - k;
-  if (o.vec) {
-    if (left > 0) v = *(const s16x8*)p;
-  } else {
-    #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) v[i] = *(const short*)(p + i);
-  }
-  return v;
-}
-
-// A tile of B rows and 64 k in LDS, 16 bytes a piece.
-// k contiguous: row r has 8 pieces, piece q at q ^ (r & 7): 8 lanes that read one q of 8 rows meet 8 places.
-// rows contiguous: line k has B/8 pieces. The transposing read of one instruction touches lines
-// {0..3} + 8g (g = 0..3), 32 bytes of each: pairs of pieces are moved by the line so that these lie apart.
-template <int B, bool ROWS>
+// A tile of B rows and 64 k in LDS, pieces of 16 bytes, one after another as lanes load them: which piece of
+// the operand a place holds is turned, so that what one instruction reads lies on different banks.
+// k contiguous: row r has 8 places; place q holds piece q ^ key(r), and the 8 rows that are read together have
+// 8 keys: neighbours (DEALT false), or 0-3 and 8-11 of every 16 (the rows of a dealt fragment).
+// rows contiguous: line k has B/8 places. The transposing read of one instruction touches lines {0..3} + 8g
+// (g = 0..3): pairs of pieces are moved by the line.
+template <int B, bool ROWS, bool DEALT>
 struct Lds {
   static constexpr int kPieces = B * BK / 8;
-  static __device__ __forceinline__ void place(int c, int& row, int& k) {
-    if (ROWS) { k = c / (B / 8); row = (c % (B / 8)) * 8; }
-    else { row = c / 8; k = (c % 8) * 8; }
+  static __device__ __forceinline__ int key(int row) {
+    return DEALT ? (row & 3) | ((row >> 1) & 4) : row & 7;
   }
   static __device__ __forceinline__ int turn(int k) { return ((k & 3) | ((k >> 1) & 4)) & (B / 16 - 1); }
-  static __device__ __forceinline__ int at(int c) {     // in shorts
+  // what the place c holds
+  static __device__ __forceinline__ void held(int c, int& row, int& k) {
     if (ROWS) {
-      const int k = c / (B / 8), p = c % (B / 8);
-      return k * B + (((p >> 1) ^ turn(k)) * 2 + (p & 1)) * 8;
+      const int p = c % (B / 8);
+      k = c / (B / 8);
+      row = (((p >> 1) ^ turn(k)) * 2 + (p & 1)) * 8;
+    } else {
+      row = c / 8;
+      k = ((c % 8) ^ key(row)) * 8;
     }
-    const int row = c / 8, q = c % 8;
-    return row * BK + ((q ^ (row & 7)) * 8);
   }
-  // fragment of 16 rows from row0, 32 k from k0: lane has row lane%16, k (lane/16)*8 .. +7
-  static __device__ __forceinline__ s16x8 fragment(short* lds, int row0, int k0, int lane) {
+  // Fragment j of 16 rows of a wave's tile that starts at row0, 32 k from k0: lane i = lane%16 has k
+  // (lane/16)*8 .. +7 of row i of the fragment. Fragments are 16 neighbouring rows, or (DEALT) of 32 rows
+  // those 8a + 4(j%2) + b for row i = 4a + b: two fragments' results are then 8 neighbours a lane.
+  static __device__ __forceinline__ s16x8 fragment(const short* lds, int row0, int j, int k0, int lane) {
+    const int i = lane & 15;
     if (!ROWS) {
-      const int row = row0 + (lane & 15), q = k0 / 8 + (lane >> 4);
-      return *(const s16x8*)(lds + row * BK + ((q ^ (row & 7)) * 8));
+      const int row = DEALT ? row0 + (j >> 1) * 32 + (i >> 2) * 8 + (j & 1) * 4 + (i & 3) : row0 + j * 16 + i;
+      const int q = k0 / 8 + (lane >> 4);
+      return *(const s16x8*)(lds + row * BK + ((q ^ key(row)) * 8));
     }
-    const int i = lane & 15, k = k0 + (lane >> 4) * 8 + (i >> 2);
+    // lane i of 16 addresses 4 rows (i%4) of line i/4 and is given row i of the 4 lines
+    const int k = k0 + (lane >> 4) * 8 + (i >> 2);
+    const int row = DEALT ? row0 + (j >> 1) * 32 + (i & 3) * 8 + (j & 1) * 4 : row0 + j * 16 + (i & 3) * 4;
     typedef __attribute__((address_space(3))) s16x4* lds4;
-    auto word = [&](int kk) {
-      return lds + kk * B + ((row0 / 16) ^ turn(kk)) * 16 + (i & 3) * 4;
-    };
+    auto word = [&](int kk) { return lds + kk * B + (((row >> 4) ^ turn(kk)) << 4) + (row & 15); };
     s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)word(k));
     s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)word(k + 4));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
 
+// Pieces of a tile on their way to LDS: N a thread
+template <int B, bool ROWS, bool DEALT, int THREADS>
+struct Loader {
+  typedef Lds<B, ROWS, DEALT> L;
+  static constexpr int N = L::kPieces / THREADS;
+  const char* base;
+  int64_t left;         // bytes from base to the operand's end
+  uint32_t off[N];      // where a piece starts; out of any range for rows that are not there
+  int k[N];
+  int kdim;
+  int64_t line;         // bytes from one k to the next where rows are contiguous
+
+  __device__ __forceinline__ Loader(const Operand& o, int row0, int tid) {
+    const int64_t start = ROWS ? row0 : row0 * o.ld;
+    base = (const char*)(o.p + start);
+    left = ((int64_t)(ROWS ? o.kdim : o.rows) * o.ld - start) * 2;
+    kdim = o.kdim;
+    line = o.ld * 2;
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      int row, kk;
+      L::held(tid + i * THREADS, row, kk);
+      k[i] = kk;
+      off[i] = ROWS ? (uint32_t)(kk * o.ld + row) * 2 : (uint32_t)(row * o.ld + kk) * 2;
+      if (row0 + row >= o.rows) off[i] = 0xffffffffu;
+    }
+  }
+  // the pieces of k0 .. k0+63 to lds. Reads behind the operand's end give zeros; so do k that are not there.
+  __device__ __forceinline__ void operator()(int k0, short* lds, int wave) const {
+    const int64_t skip = ROWS ? k0 * line : (int64_t)k0 * 2;
+    const int64_t rest = left - skip;
+    const uint32_t bytes = rest > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)rest;
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + skip), 0, bytes, 0x00020000);
+    typedef __attribute__((address_space(3))) void* lds_t;
+    #pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t at = off[i];
+      if (!ROWS && k0 + k[i] >= kdim) at = 0xffffffffu;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + (i * THREADS + wave * 64) * 8), 16, at, 0, 0, 0);
+    }
+  }
+};
+
 // Workgroups that share operand rows run one after another on one XCD and find them in its L2.
-__device__ __forceinline__ int xcd_order(int wg, int n) {
-  const int q = n / 8, rem = n % 8, xcd = wg % 8, i = wg / 8;
+__device__ __forceinline__ uint32_t xcd_order(uint32_t wg, uint32_t n) {
+  const uint32_t q = n / 8, rem = n % 8, xcd = wg % 8, i = wg / 8;
   return xcd < rem ? xcd * (q + 1) + i : rem * (q + 1) + (xcd - rem) * q + i;
 }
 
 // ------------------------------------------------------------ the product in 16 bits
 
 template <typename T, bool PR, bool QR, int BM, int BN>
-__global__ __launch_bounds__(256) void product_kernel(Operand<T> P, Operand<T> Q, Epilogue<T> epi,
+__global__ __launch_bounds__(256) void product_kernel(Operand P, Operand Q, Epilogue<T> epi,
                                                       float* __restrict__ part, int tiles_m,
                                                       int tiles_n, int splits) {
   constexpr int FM = BM / 32, FN = BN / 32;         // fragments of a wave: 2 x 2 waves
-  constexpr int NP = Lds<BM, PR>::kPieces / 256, NQ = Lds<BN, QR>::kPieces / 256;
-  __shared__ __align__(16) short lds_p[2][BM * BK];
-  __shared__ __align__(16) short lds_q[2][BN * BK];
-  const int id = xcd_order((int)blockIdx.x, tiles_m * tiles_n * splits);
-  const int tn = id % tiles_n, tm = id / tiles_n % tiles_m, sp = id / tiles_n / tiles_m;
+  typedef Loader<BM, PR, false, 256> LP;
+  typedef Loader<BN, QR, true, 256> LQ;
+  // two buffers, named apart: what fills one is then known not to touch the other
+  __shared__ __align__(16) short p0[BM * BK], p1[BM * BK], q0[BN * BK], q1[BN * BK];
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x), id_m = id / (uint32_t)tiles_n,
+                 sp = id_m / (uint32_t)tiles_m;
+  const int tn = (int)(id - id_m * tiles_n), tm = (int)(id_m - sp * tiles_m);
   const int m0 = tm * BM, n0 = tn * BN;
   const int steps = (P.kdim + BK - 1) / BK;
   const int s0 = (int)((int64_t)steps * sp / splits), s1 = (int)((int64_t)steps * (sp + 1) / splits);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
-
-  s16x8 rp[NP], rq[NQ];
-  auto fetch = [&](int s) {
-    #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      int row, k;
-      Lds<BM, PR>::place(tid + i * 256, row, k);
-      rp[i] = load8<T, PR>(P, m0 + row, s * BK + k);
-    }
-    #pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      int row, k;
-      Lds<BN, QR>::place(tid + i * 256, row, k);
-      rq[i] = load8<T, QR>(Q, n0 + row, s * BK + k);
-    }
-  };
-  auto put = [&](int buf) {
-    #pragma unroll
-    for (int i = 0; i < NP; ++i) *(s16x8*)(lds_p[buf] + Lds<BM, PR>::at(tid + i * 256)) = rp[i];
-    #pragma unroll
-    for (int i = 0; i < NQ; ++i) *(s16x8*)(lds_q[buf] + Lds<BN, QR>::at(tid + i * 256)) = rq[i];
-  };
+  const int M = P.rows, N = Q.rows;
+  const LP load_p(P, m0, tid);
+  const LQ load_q(Q, n0, tid);
 
   f32x4 acc[FM][FN];
   #pragma unroll
@@ -270,65 +324,124 @@ __global__ __launch_bounds__(256) void product_kernel(Operand<T> P, Operand<T> Q
     #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-  if (s0 < s1) {
-    fetch(s0);
-    put(0);
-    if (s0 + 1 < s1) fetch(s0 + 1);
-  }
-  __syncthreads();
-  for (int s = s0; s < s1; ++s) {
-    const int buf = (s - s0) & 1;
-    if (s + 1 < s1) {
-      put(buf ^ 1);                       // its readers are behind the last barrier
-      if (s + 2 < s1) fetch(s + 2);
+  auto fill = [&](int s, short* p, short* q) {
+    if (s < s1) {
+      load_p(s * BK, p, wave);
+      load_q(s * BK, q, wave);
     }
+  };
+  // what was asked for has come, here and in the other waves; and they have read the other buffer
+  auto meet = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  auto multiply = [&](const short* p, const short* q) {
     #pragma unroll
     for (int k = 0; k < BK; k += 32) {
       s16x8 fp[FM], fq[FN];
       #pragma unroll
-      for (int i = 0; i < FM; ++i) fp[i] = Lds<BM, PR>::fragment(lds_p[buf], wm + i * 16, k, lane);
+      for (int j = 0; j < FN; ++j) fq[j] = LQ::L::fragment(q, wn, j, k, lane);
       #pragma unroll
-      for (int j = 0; j < FN; ++j) fq[j] = Lds<BN, QR>::fragment(lds_q[buf], wn + j * 16, k, lane);
+      for (int i = 0; i < FM; ++i) fp[i] = LP::L::fragment(p, wm, i, k, lane);
       #pragma unroll
       for (int i = 0; i < FM; ++i)
         #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
     }
-    __syncthreads();
+  };
+  fill(s0, p0, q0);
+  for (int s = s0; s < s1; s += 2) {
+    meet();
+    fill(s + 1, p1, q1);
+    multiply(p0, q0);
+    if (s + 1 >= s1) break;
+    meet();
+    fill(s + 2, p0, q0);
+    multiply(p1, q1);
   }
-  // lane: output row lane%16 of a fragment, columns (lane/16)*4 .. +3
-  const int M = P.rows, N = Q.rows;
-  #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int64_t m = (int64_t)m0 + wm + i * 16 + (lane & 15);
-    if (m >= M) continue;
+
+  // lane: output row lane%16 of a fragment; of fragments j, j+1 columns (lane/16)*8 + 0..3 and + 4..7
+  const int mine = n0 + wn + (lane >> 4) * 8;
+  auto each = [&](auto f) {
     #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (splits == 1) epi(m, n, N, acc[i][j]);
-      else if (n < N) store4(part + ((int64_t)sp * M + m) * N + n, N - n, epi.vec, acc[i][j]);
+    for (int j = 0; j < FN; j += 2) {
+      const int n = mine + j * 16;
+      if (n >= N) continue;
+      #pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int64_t m = (int64_t)m0 + wm + i * 16 + (lane & 15);
+        if (m < M) f(m, n, i, j);
+      }
     }
+  };
+  if (splits > 1) {
+    each([&](int64_t m, int n, int i, int j) {
+      float* to = part + ((int64_t)sp * M + m) * N + n;
+      store4(to, N - n, epi.vec, acc[i][j]);
+      store4(to + 4, N - n - 4, epi.vec, acc[i][j + 1]);
+    });
+  } else if (epi.vec) {
+    f32x8 bias[FN / 2];
+    #pragma unroll
+    for (int j = 0; j < FN; j += 2)
+      bias[j / 2] = epi.bias && mine + j * 16 < N ? widen8<T>(*(const s16x8*)(epi.bias + mine + j * 16)) : f32x8{};
+    by_act(epi.act, [&](auto A) {
+      each([&](int64_t m, int n, int i, int j) {
+        epi.template eight<A.value>(m * N + n, __builtin_shufflevector(acc[i][j], acc[i][j + 1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                    bias[j / 2]);
+      });
+    });
+  } else {
+    by_act(epi.act, [&](auto A) {
+      each([&](int64_t m, int n, int i, int j) {
+        epi.template four<A.value>(m, n, N, acc[i][j]);
+        epi.template four<A.value>(m, n + 4, N, acc[i][j + 1]);
+      });
+    });
+  }
+}
+
+// lines of `from` values into lines of `to`, a multiple of 8, with zeros behind
+__global__ __launch_bounds__(256) void widen_lines_kernel(const short* __restrict__ in, short* __restrict__ out,
+                                                          int64_t lines, int from, int to) {
+  const int pieces = to / 8;
+  const int64_t total = lines * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t l = i / pieces;
+    const int c = (int)(i - l * pieces) * 8;
+    s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    #pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < from) v[e] = in[l * from + c + e];
+    *(s16x8*)(out + i * 8) = v;
   }
 }
 
 // ------------------------------------------------------------ the product in 32 bits
 
+struct OperandF32 {
+  const float* p;
+  int rows, kdim;
+  int64_t ld;
+};
+
 // 64 x 64 tiles, 16 k a step; LDS lines hold one k (a lane of the matrix instruction has one k of one row)
 template <bool PR, bool QR>
-__global__ __launch_bounds__(256) void product_f32_kernel(Operand<float> P, Operand<float> Q,
+__global__ __launch_bounds__(256) void product_f32_kernel(OperandF32 P, OperandF32 Q,
                                                           Epilogue<float> epi, float* __restrict__ part,
                                                           int tiles_m, int tiles_n, int splits) {
   constexpr int B = 64, K = 16, LD = B + 4;
   __shared__ float lp[2][K][LD], lq[2][K][LD];
-  const int id = xcd_order((int)blockIdx.x, tiles_m * tiles_n * splits);
-  const int tn = id % tiles_n, tm = id / tiles_n % tiles_m, sp = id / tiles_n / tiles_m;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x), id_m = id / (uint32_t)tiles_n,
+                 sp = id_m / (uint32_t)tiles_m;
+  const int tn = (int)(id - id_m * tiles_n), tm = (int)(id_m - sp * tiles_m);
   const int m0 = tm * B, n0 = tn * B;
   const int steps = (P.kdim + K - 1) / K;
   const int s0 = (int)((int64_t)steps * sp / splits), s1 = (int)((int64_t)steps * (sp + 1) / splits);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
   float rp[4], rq[4];
-  auto one = [](const Operand<float>& o, bool rows, int row, int k) {
+  auto one = [](const OperandF32& o, bool rows, int row, int k) {
     if (row >= o.rows || k >= o.kdim) return 0.0f;
     return rows ? o.p[(int64_t)k * o.ld + row] : o.p[(int64_t)row * o.ld + k];
   };
@@ -389,17 +502,19 @@ __global__ __launch_bounds__(256) void product_f32_kernel(Operand<float> P, Oper
     __syncthreads();
   }
   const int M = P.rows, N = Q.rows;
-  #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = (int64_t)m0 + wm + i * 16 + (lane & 15);
-    if (m >= M) continue;
+  by_act(epi.act, [&](auto A) {
     #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (splits == 1) epi(m, n, N, acc[i][j]);
-      else if (n < N) store4(part + ((int64_t)sp * M + m) * N + n, N - n, epi.vec, acc[i][j]);
+    for (int i = 0; i < 2; ++i) {
+      const int64_t m = (int64_t)m0 + wm + i * 16 + (lane & 15);
+      if (m >= M) continue;
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+        if (splits == 1) epi.template four<A.value>(m, n, N, acc[i][j]);
+        else if (n < N) store4(part + ((int64_t)sp * M + m) * N + n, N - n, epi.vec, acc[i][j]);
+      }
     }
-  }
+  });
 }
 
 // the parts of a split product, added in order, and its epilogue
@@ -408,18 +523,21 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
                                                    int64_t M, int N, int splits) {
   const int n4 = (N + 3) / 4;
   const int64_t total = M * n4, plane = M * N;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / n4;
-    const int n = (int)(i - m * n4) * 4;
-    f32x4 v = {0, 0, 0, 0};
-    for (int s = 0; s < splits; ++s) v += load4(part + s * plane + m * N + n, N - n, epi.vec);
-    epi(m, n, N, v);
-  }
+  by_act(epi.act, [&](auto A) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+      const int64_t m = i / n4;
+      const int n = (int)(i - m * n4) * 4;
+      f32x4 v = {0, 0, 0, 0};
+      #pragma unroll 4
+      for (int s = 0; s < splits; ++s) v += load4(part + s * plane + m * N + n, N - n, epi.vec);
+      epi.template four<A.value>(m, n, N, v);
+    }
+  });
 }
 
 // ------------------------------------------------------------ dz and its column sums
 
-// dz = dy act'(z) where dz is given; sums over a chunk of rows to part[chunk][N] where part is given.
+// dz = dy act'(z), unless act is none; sums over a chunk of rows to part[chunk][N] where part is given.
 // A thread has VEC columns, a workgroup a tile of columns and a chunk of rows.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ z,
@@ -437,38 +555,32 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
   float acc[VEC];
   #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-  if (on) {
-    #pragma unroll 4
-    for (int64_t m = m0 + r; m < m1; m += rows) {
-      const int64_t at = m * N + c0 + v * VEC;
-      if constexpr (VEC == 1) {
-        float d = Num<T>::get(dy + at);
-        if (dz) {
-          d *= act_slope(Num<T>::get(z + at), act);
-          Num<T>::put(dz + at, d);
-        }
-        acc[0] += d;
-      } else {
-        constexpr int H = VEC / 4;
-        f32x4 d[H], zz[H];
+  if (on)
+    by_act(act, [&](auto A) {
+      #pragma unroll 4
+      for (int64_t m = m0 + r; m < m1; m += rows) {
+        const int64_t at = m * N + c0 + v * VEC;
+        constexpr int H = VEC == 1 ? 1 : VEC / 4, E = VEC == 1 ? 1 : 4;
+        f32x4 d[H];
         #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          d[h] = load4(dy + at + 4 * h, 4, true);
-          if (dz) zz[h] = load4(z + at + 4 * h, 4, true);
-        }
-        #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          if (dz) {
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) d[h][i] *= act_slope(zz[h][i], act);
-            store4(dz + at + 4 * h, 4, true, d[h]);
-          }
+        for (int h = 0; h < H; ++h) d[h] = load4(dy + at + 4 * h, E, VEC > 1);
+        if constexpr (A.value != ACT_NONE) {
+          f32x4 zz[H];
           #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[4 * h + i] += d[h][i];
+          for (int h = 0; h < H; ++h) zz[h] = load4(z + at + 4 * h, E, VEC > 1);
+          #pragma unroll
+          for (int h = 0; h < H; ++h) {
+            #pragma unroll
+            for (int i = 0; i < E; ++i) d[h][i] *= act_slope<A.value>(zz[h][i]);
+            store4(dz + at + 4 * h, E, VEC > 1, d[h]);
+          }
         }
+        #pragma unroll
+        for (int h = 0; h < H; ++h)
+          #pragma unroll
+          for (int i = 0; i < E; ++i) acc[E * h + i] += d[h][i];
       }
-    }
-  }
+    });
   if (!part) return;
   if (on)
     #pragma unroll
@@ -512,31 +624,43 @@ void by_type(torch::ScalarType t, F f) {
   else TORCH_CHECK(false, "linear_act: fp32, bf16 and fp16 are taken");
 }
 
-template <typename T>
-Operand<T> operand(const torch::Tensor& t, bool rows_contiguous) {
-  Operand<T> o;
-  o.p = (const T*)t.data_ptr();
+// t as an operand; `keep` holds a copy with wider lines where t's do not start at 16 bytes
+Operand operand(const torch::Tensor& t, bool rows_contiguous, torch::Tensor& keep, hipStream_t stream) {
+  Operand o;
   o.rows = (int)t.size(rows_contiguous ? 1 : 0);
   o.kdim = (int)t.size(rows_contiguous ? 0 : 1);
   o.ld = t.size(1);
-  o.vec = t.size(1) % 8 == 0 && aligned(o.p, 16);
+  keep = t;
+  if (o.ld % 8 != 0 || !aligned(t.data_ptr(), 16)) {
+    o.ld = (o.ld + 7) / 8 * 8;
+    keep = torch::empty({t.size(0), o.ld}, t.options());
+    const int64_t pieces = t.size(0) * o.ld / 8;
+    hipLaunchKernelGGL(widen_lines_kernel, dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 8192)),
+                       dim3(256), 0, stream, (const short*)t.data_ptr(), (short*)keep.data_ptr(), t.size(0),
+                       (int)t.size(1), (int)o.ld);
+  }
+  o.p = (const short*)keep.data_ptr();
   return o;
+}
+
+OperandF32 operand_f32(const torch::Tensor& t, bool rows_contiguous) {
+  return {t.data_ptr<float>(), (int)t.size(rows_contiguous ? 1 : 0), (int)t.size(rows_contiguous ? 0 : 1),
+          t.size(1)};
 }
 
 // D[m][n] = sum_k P(m,k) Q(n,k), with the epilogue
 template <typename T, bool PR, bool QR>
 void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hipStream_t stream) {
-  const Operand<T> P = operand<T>(p, PR), Q = operand<T>(q, QR);
-  const int64_t M = P.rows, N = Q.rows, K = P.kdim;
-  epi.vec = N % 4 == 0 && aligned(epi.y, 4 * sizeof(T)) && (!epi.z || aligned(epi.z, 4 * sizeof(T)))
-            && (!epi.res || aligned(epi.res, 4 * sizeof(T)))
-            && (!epi.bias || aligned(epi.bias, 4 * sizeof(T)));
+  const int64_t M = p.size(PR ? 1 : 0), N = q.size(QR ? 1 : 0), K = p.size(PR ? 0 : 1);
+  constexpr int W = sizeof(T) == 2 ? 8 : 4;
+  epi.vec = N % W == 0 && aligned(epi.y, 16) && (!epi.z || aligned(epi.z, 16))
+            && (!epi.res || aligned(epi.res, 16)) && (!epi.bias || aligned(epi.bias, 16));
   int BM = 64, BN = 64, step = 16;
   if constexpr (sizeof(T) == 2) {
     step = BK;
     auto tiles = [&](int64_t a, int64_t b) { return ((M + a - 1) / a) * ((N + b - 1) / b); };
-    if (M > 64 && tiles(128, 64) >= 256) BM = 128;
-    if (BM == 128 && N > 64 && tiles(128, 128) >= 256) BN = 128;
+    if (M > 64 && (tiles(128, 64) >= 256 || K >= 8192)) BM = 128;
+    if (BM == 128 && N > 64 && (tiles(128, 128) >= 256 || K >= 8192)) BN = 128;
   }
   const int64_t tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, steps = (K + step - 1) / step;
   // few tiles and a long k: enough parts for 2 workgroups a CU, each with 4 steps at least
@@ -550,17 +674,18 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
     part = ws.data_ptr<float>();
   }
   const dim3 grid((unsigned)(tm * tn * splits)), block(256);
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, block, 0, stream, P, Q, epi, part, (int)tm, (int)tn, (int)splits);
-  };
   if constexpr (sizeof(T) == 4) {
-    go(product_f32_kernel<PR, QR>);
-  } else if (BM == 128 && BN == 128) {
-    go(product_kernel<T, PR, QR, 128, 128>);
-  } else if (BM == 128) {
-    go(product_kernel<T, PR, QR, 128, 64>);
+    hipLaunchKernelGGL((product_f32_kernel<PR, QR>), grid, block, 0, stream, operand_f32(p, PR),
+                       operand_f32(q, QR), epi, part, (int)tm, (int)tn, (int)splits);
   } else {
-    go(product_kernel<T, PR, QR, 64, 64>);
+    torch::Tensor keep_p, keep_q;
+    const Operand P = operand(p, PR, keep_p, stream), Q = operand(q, QR, keep_q, stream);
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, grid, block, 0, stream, P, Q, epi, part, (int)tm, (int)tn, (int)splits);
+    };
+    if (BM == 128 && BN == 128) go(product_kernel<T, PR, QR, 128, 128>);
+    else if (BM == 128) go(product_kernel<T, PR, QR, 128, 64>);
+    else go(product_kernel<T, PR, QR, 64, 64>);
   }
   if (splits > 1) {
     const int64_t work = M * ((N + 3) / 4);
@@ -604,8 +729,9 @@ void check(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& 
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && w.dim() == 2 && x.is_contiguous() && w.is_contiguous(),
               "linear_act: x [M,K] and weight [N,K], contiguous");
   TORCH_CHECK(x.size(1) == w.size(1) && x.size(1) > 0 && w.size(0) > 0, "linear_act: sizes");
-  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 256 && x.size(1) < (1 << 30) && w.size(0) < (1 << 30),
-              "linear_act: a dimension is too large");
+  // offsets in a tile of 128 lines, or of 64 lines of 128, are 32 bits
+  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 256 && x.size(1) <= (1 << 23) && w.size(0) <= (1 << 23),
+              "linear_act: 2^31 rows or more, or more than 2^23 columns");
   TORCH_CHECK(w.scalar_type() == x.scalar_type() && w.device() == x.device(), "linear_act: weight");
   TORCH_CHECK(!b.defined() || (b.is_contiguous() && b.dim() == 1 && b.size(0) == w.size(0)
               && b.scalar_type() == x.scalar_type() && b.device() == x.device()), "linear_act: bias");
