@@ -141,48 +141,57 @@ __device__ __forceinline__ uint32_t to_e4m3(f32x4 v) {
 
 // ------------------------------------------------------------------ norm
 
-// part[block] = sum of squares of the block's chunks, added in a fixed order
+__device__ __forceinline__ double wave_sum(double v) {
+  #pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// part[block] = sum of squares of the block's chunks, added in a fixed order. 16 values are added in fp32, all
+// else in 64 bits: an error of the norm would move every gradient the same way, and 8-bit moments over a border.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(
     const int64_t* __restrict__ rows, const int* __restrict__ chunks, int n_chunks,
-    float* __restrict__ part) {
-  __shared__ float lds[kThreads / FAA_WAVE];
-  float acc = 0.0f;
+    double* __restrict__ part) {
+  __shared__ double lds[kThreads / FAA_WAVE];
+  double acc = 0.0;
   for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
     Row r = read_row(rows, chunks[2 * c]);
     if (r.g == nullptr) continue;
     int64_t base = (int64_t)chunks[2 * c + 1] * kChunk + threadIdx.x * 4;
+    float s = 0.0f;
     #pragma unroll
     for (int it = 0; it < kIters; ++it) {
       f32x4 g = load4((const T*)r.g, base + it * kThreads * 4, r.n, r.aligned);
-      acc += g[0] * g[0] + g[1] * g[1] + g[2] * g[2] + g[3] * g[3];
+      s += (g[0] * g[0] + g[1] * g[1]) + (g[2] * g[2] + g[3] * g[3]);
     }
+    acc += (double)s;
   }
-  acc = faa_block_reduce_sum(acc, lds);
-  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+  acc = wave_sum(acc);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
 // scal = {clip factor, 1/(1-b1^t), 1/sqrt(1-b2^t)} of the step that begins
 __global__ __launch_bounds__(kThreads) void adamw_begin_kernel(
-    const float* __restrict__ part, int n_part, int64_t* __restrict__ step,
+    const double* __restrict__ part, int n_part, int64_t* __restrict__ step,
     float* __restrict__ scal, double b1, double b2, float clip) {
-  __shared__ double lds[kThreads];
+  __shared__ double lds[kThreads / FAA_WAVE];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n_part; i += kThreads) s += (double)part[i];
-  lds[threadIdx.x] = s;
+  #pragma unroll 4
+  for (int i = threadIdx.x; i < n_part; i += kThreads) s += part[i];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = s;
+  // the powers are taken by other waves meanwhile
+  if (threadIdx.x == 64) scal[1] = (float)(1.0 / (1.0 - pow(b1, (double)(step[0] + 1))));
+  if (threadIdx.x == 128) scal[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)(step[0] + 1))));
   __syncthreads();
-  for (int w = kThreads / 2; w > 0; w >>= 1) {
-    if ((int)threadIdx.x < w) lds[threadIdx.x] += lds[threadIdx.x + w];
-    __syncthreads();
-  }
   if (threadIdx.x == 0) {
-    int64_t t = step[0] + 1;
-    step[0] = t;
-    float norm = (float)sqrt(lds[0]);
+    step[0] += 1;
+    float norm = (float)sqrt(lds[0] + lds[1] + lds[2] + lds[3]);
     scal[0] = clip > 0.0f ? fminf(1.0f, clip / (norm + 1e-6f)) : 1.0f;
     if (norm != norm) scal[0] = norm;     // fminf would hide a norm that is no number
-    scal[1] = (float)(1.0 / (1.0 - pow(b1, (double)t)));
-    scal[2] = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
   }
 }
 
@@ -309,7 +318,7 @@ void adamw_step(std::vector<torch::Tensor> rows, std::vector<torch::Tensor> chun
               "adamw_step: moments are fp32, or e4m3 with a scale for every block of 256");
   TORCH_CHECK(step.scalar_type() == torch::kInt64 && scal.numel() >= 3
               && scal.scalar_type() == torch::kFloat32 && lr.scalar_type() == torch::kFloat32
-              && part.scalar_type() == torch::kFloat32, "adamw_step: scalars");
+              && part.scalar_type() == torch::kFloat64, "adamw_step: scalars");
   const c10::OptionalDeviceGuard guard(m.device());
   auto stream = at::hip::getCurrentHIPStream().stream();
   const int per = rows.empty() ? 0 : (int)(part.numel() / (int64_t)rows.size());
@@ -325,7 +334,7 @@ void adamw_step(std::vector<torch::Tensor> rows, std::vector<torch::Tensor> chun
     if (clip <= 0.0 || chunks[i].size(0) == 0) continue;
     const int nc = (int)chunks[i].size(0), grid = std::min(nc, per);
     TORCH_CHECK(grid > 0, "adamw_step: part is too short");
-    float* out = part.data_ptr<float>() + n_part;
+    double* out = part.data_ptr<double>() + n_part;
     auto go = [&](auto kern) {
       hipLaunchKernelGGL(kern, dim3(grid), dim3(kThreads), 0, stream,
                          rows[i].data_ptr<int64_t>(), chunks[i].data_ptr<int>(), nc, out);
@@ -336,7 +345,7 @@ void adamw_step(std::vector<torch::Tensor> rows, std::vector<torch::Tensor> chun
     n_part += grid;
   }
   hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(kThreads), 0, stream,
-                     part.data_ptr<float>(), n_part, step.data_ptr<int64_t>(),
+                     part.data_ptr<double>(), n_part, step.data_ptr<int64_t>(),
                      scal.data_ptr<float>(), b1, b2, (float)clip);
   Moments st{m.data_ptr(), r.data_ptr(), bits == 8 ? m_scale.data_ptr<float>() : nullptr,
              bits == 8 ? r_scale.data_ptr<float>() : nullptr};

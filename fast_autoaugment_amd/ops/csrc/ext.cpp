@@ -72,6 +72,22 @@ torch::Tensor dwconv_bwd_data(torch::Tensor dy, torch::Tensor w, int64_t stride,
 torch::Tensor dwconv_bwd_weight(torch::Tensor dy, torch::Tensor x, int64_t stride,
                                 int64_t pt, int64_t pl, int64_t KH, int64_t KW);
 
+// what device tables of addresses depend on: place, size and memory order of every tensor and of its gradient
+static py::bytes tensor_addresses(const std::vector<torch::Tensor>& ts) {
+  std::vector<int64_t> a;
+  a.reserve(ts.size() * 16);
+  for (const auto& t : ts) {
+    a.push_back((int64_t)t.data_ptr());
+    a.insert(a.end(), t.sizes().begin(), t.sizes().end());
+    a.insert(a.end(), t.strides().begin(), t.strides().end());
+    const auto& g = t.grad();
+    const bool strided = g.defined() && g.layout() == torch::kStrided;
+    a.push_back(strided ? (int64_t)g.data_ptr() : g.defined() ? -1 : 0);
+    if (strided) a.insert(a.end(), g.strides().begin(), g.strides().end());
+  }
+  return py::bytes((const char*)a.data(), a.size() * sizeof(int64_t));
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scale_bcast", &scale_bcast, "out = x * s[b] (per-sample broadcast)");
   m.def("scale_lerp", &scale_lerp, "out = a[b]*x1 + (1-a[b])*x2");
@@ -88,6 +104,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ema_lerp_", &ema_lerp_);
   m.def("rmsprop_fused_step_mixed", &rmsprop_fused_step_mixed,
         "fused TF-semantics RMSprop on flat mixed-precision buffers");
+  m.def("tensor_addresses", &tensor_addresses, "places and strides of tensors and of their gradients");
   m.def("adamw_step", &adamw_step,
         "AdamW over a table of tensors, moments in fp32 or in e4m3 blocks");
   m.def("gather_grads", &gather_grads,

@@ -133,8 +133,9 @@ __device__ __forceinline__ float act_slope(float z) {
   return 1.0f;
 }
 // f(activation as a constant): one branch outside the loops, not one an element
-template <typename F>
+template <bool ANY = true, typename F>
 __device__ __forceinline__ void by_act(int act, F f) {
+  if constexpr (!ANY) return f(std::integral_constant<int, ACT_NONE>{});
   if (act == ACT_SWISH) f(std::integral_constant<int, ACT_SWISH>{});
   else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
   else if (act == ACT_SIGMOID) f(std::integral_constant<int, ACT_SIGMOID>{});
@@ -175,11 +176,9 @@ struct Epilogue {
     for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(v[i]);
     store4(y + at, left, vec, v);
   }
-  // 8 columns, 16 bytes at once
+  // 8 columns, 16 bytes at once; bias and residual are in v
   template <int ACT>
-  __device__ __forceinline__ void eight(int64_t at, f32x8 v, f32x8 b) const {
-    v += b;
-    if (res) v += widen8<T>(*(const s16x8*)(res + at));
+  __device__ __forceinline__ void eight(int64_t at, f32x8 v) const {
     s16x8 out;
     if (z) {
       #pragma unroll
@@ -273,10 +272,11 @@ struct Loader {
       if (row0 + row >= o.rows) off[i] = 0xffffffffu;
     }
   }
-  // the pieces of k0 .. k0+63 to lds. Reads behind the operand's end give zeros; so do k that are not there.
-  __device__ __forceinline__ void operator()(int k0, short* lds, int wave) const {
+  // The pieces of k0 .. k0+63 to lds. Reads behind the operand's end give zeros; so do k that are not there, and
+  // all of a step that is not wanted: none of these touches memory.
+  __device__ __forceinline__ void operator()(int k0, bool wanted, short* lds, int wave) const {
     const int64_t skip = ROWS ? k0 * line : (int64_t)k0 * 2;
-    const int64_t rest = left - skip;
+    const int64_t rest = wanted ? left - skip : 0;
     const uint32_t bytes = rest > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)rest;
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + skip), 0, bytes, 0x00020000);
     typedef __attribute__((address_space(3))) void* lds_t;
@@ -297,8 +297,9 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t wg, uint32_t n) {
 
 // ------------------------------------------------------------ the product in 16 bits
 
+// Operands with contiguous rows are those of the gradients, which have no bias, residual or activation.
 template <typename T, bool PR, bool QR, int BM, int BN>
-__global__ __launch_bounds__(256) void product_kernel(Operand P, Operand Q, Epilogue<T> epi,
+__global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, Epilogue<T> epi,
                                                       float* __restrict__ part, int tiles_m,
                                                       int tiles_n, int splits) {
   constexpr int FM = BM / 32, FN = BN / 32;         // fragments of a wave: 2 x 2 waves
@@ -325,16 +326,14 @@ __global__ __launch_bounds__(256) void product_kernel(Operand P, Operand Q, Epil
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
   auto fill = [&](int s, short* p, short* q) {
-    if (s < s1) {
-      load_p(s * BK, p, wave);
-      load_q(s * BK, q, wave);
-    }
+    load_p(s * BK, s < s1, p, wave);
+    load_q(s * BK, s < s1, q, wave);
   };
-  // what was asked for has come, here and in the other waves; and they have read the other buffer
-  auto meet = [] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
+  // The older of two steps' pieces have come, here and in the other waves. Loads end in order and every step
+  // asks for as many, so a count says so; other loads in flight only make it stricter.
+  auto come = [] { asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(LP::N + LQ::N) : "memory"); };
+  // all waves have read their fragments: the buffer may be filled again
+  auto read = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
   auto multiply = [&](const short* p, const short* q) {
     #pragma unroll
     for (int k = 0; k < BK; k += 32) {
@@ -349,19 +348,43 @@ __global__ __launch_bounds__(256) void product_kernel(Operand P, Operand Q, Epil
         for (int j = 0; j < FN; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
     }
   };
-  fill(s0, p0, q0);
-  for (int s = s0; s < s1; s += 2) {
-    meet();
-    fill(s + 1, p1, q1);
-    multiply(p0, q0);
-    if (s + 1 >= s1) break;
-    meet();
-    fill(s + 2, p0, q0);
-    multiply(p1, q1);
+  const int mine = n0 + wn + (lane >> 4) * 8;       // the lane's first column
+  // the residual is on its way during the product; where there is none to read at once, zeros are read from nowhere
+  typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+  u32x4 res[FM][FN / 2];
+  if constexpr (!PR && !QR) {
+    const int64_t rest = splits == 1 && epi.vec && epi.res ? ((int64_t)M - m0) * N * 2 : 0;
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(epi.res + (int64_t)m0 * N), 0,
+                                                  rest > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)rest, 0x00020000);
+    #pragma unroll
+    for (int i = 0; i < FM; ++i)
+      #pragma unroll
+      for (int j = 0; j < FN; j += 2) {
+        const uint32_t at = (uint32_t)((wm + i * 16 + (lane & 15)) * N + mine + j * 16) * 2;
+        res[i][j / 2] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, mine + j * 16 < N ? at : 0xffffffffu, 0, 0);
+      }
   }
+  fill(s0, p0, q0);
+  fill(s0 + 1, p1, q1);
+  int s = s0;
+  for (; s + 2 < s1; s += 2) {
+    come();
+    multiply(p0, q0);
+    read();
+    fill(s + 2, p0, q0);
+    come();
+    multiply(p1, q1);
+    read();
+    fill(s + 3, p1, q1);
+  }
+  if (s < s1) {     // one or two steps are left; no others are asked for
+    come();
+    multiply(p0, q0);
+  }
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  if (s + 1 < s1) multiply(p1, q1);
 
   // lane: output row lane%16 of a fragment; of fragments j, j+1 columns (lane/16)*8 + 0..3 and + 4..7
-  const int mine = n0 + wn + (lane >> 4) * 8;
   auto each = [&](auto f) {
     #pragma unroll
     for (int j = 0; j < FN; j += 2) {
@@ -384,15 +407,16 @@ __global__ __launch_bounds__(256) void product_kernel(Operand P, Operand Q, Epil
     f32x8 bias[FN / 2];
     #pragma unroll
     for (int j = 0; j < FN; j += 2)
-      bias[j / 2] = epi.bias && mine + j * 16 < N ? widen8<T>(*(const s16x8*)(epi.bias + mine + j * 16)) : f32x8{};
-    by_act(epi.act, [&](auto A) {
+      bias[j / 2] = !PR && !QR && epi.bias && mine + j * 16 < N ? widen8<T>(*(const s16x8*)(epi.bias + mine + j * 16)) : f32x8{};
+    by_act<!PR && !QR>(epi.act, [&](auto A) {
       each([&](int64_t m, int n, int i, int j) {
-        epi.template eight<A.value>(m * N + n, __builtin_shufflevector(acc[i][j], acc[i][j + 1], 0, 1, 2, 3, 4, 5, 6, 7),
-                                    bias[j / 2]);
+        f32x8 v = __builtin_shufflevector(acc[i][j], acc[i][j + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        if constexpr (!PR && !QR) v += widen8<T>(__builtin_bit_cast(s16x8, res[i][j / 2]));
+        epi.template eight<A.value>(m * N + n, v + bias[j / 2]);
       });
     });
   } else {
-    by_act(epi.act, [&](auto A) {
+    by_act<!PR && !QR>(epi.act, [&](auto A) {
       each([&](int64_t m, int n, int i, int j) {
         epi.template four<A.value>(m, n, N, acc[i][j]);
         epi.template four<A.value>(m, n + 4, N, acc[i][j + 1]);
@@ -537,11 +561,11 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 
 // ------------------------------------------------------------ dz and its column sums
 
-// dz = dy act'(z), unless act is none; sums over a chunk of rows to part[chunk][N] where part is given.
+// dz = dy act'(z), unless act is none; sums over a chunk of rows to part[chunk][N], or of all rows to db.
 // A thread has VEC columns, a workgroup a tile of columns and a chunk of rows.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ z,
-                                                    T* __restrict__ dz, float* __restrict__ part,
+                                                    T* __restrict__ dz, float* __restrict__ part, T* __restrict__ db,
                                                     int64_t M, int N, int tile, int ntile, int chunk,
                                                     int act) {
   __shared__ float lds[256 * VEC];
@@ -581,33 +605,41 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
           for (int i = 0; i < E; ++i) acc[E * h + i] += d[h][i];
       }
     });
-  if (!part) return;
+  if (!part && !db) return;
   if (on)
     #pragma unroll
     for (int j = 0; j < VEC; ++j) lds[r * cols + v * VEC + j] = acc[j];
   __syncthreads();
   for (int c = threadIdx.x; c < cols; c += 256) {
     float s = 0.0f;
+    #pragma unroll 4
     for (int q = 0; q < rows; ++q) s += lds[q * cols + c];
-    part[ck * N + c0 + c] = s;
+    if (db) Num<T>::put(db + c0 + c, s);
+    else part[ck * N + c0 + c] = s;
   }
 }
 
-// out[n] = sum over the chunks, 32 columns a workgroup
+// out[n] = sum over the chunks, 8 columns a workgroup: a few loads a thread
 template <typename T>
 __global__ __launch_bounds__(1024) void column_join_kernel(const float* __restrict__ part, int64_t chunks,
                                                            int N, T* __restrict__ out) {
-  __shared__ float lds[32][33];
-  const int col = threadIdx.x & 31, row = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
+  __shared__ float lds[128][9];
+  const int col = threadIdx.x & 7, row = threadIdx.x >> 3, n = blockIdx.x * 8 + col;
   float s = 0.0f;
   if (n < N)
-    for (int64_t r = row; r < chunks; r += 32) s += part[r * N + n];
+    #pragma unroll 4
+    for (int64_t r = row; r < chunks; r += 128) s += part[r * N + n];
   lds[row][col] = s;
   __syncthreads();
+  #pragma unroll
+  for (int w = 64; w >= 8; w >>= 1) {
+    if (row < w) lds[row][col] += lds[row + w][col];
+    __syncthreads();
+  }
   if (row == 0 && n < N) {
     s = 0.0f;
     #pragma unroll
-    for (int r = 0; r < 32; ++r) s += lds[r][col];
+    for (int r = 0; r < 8; ++r) s += lds[r][col];
     Num<T>::put(out + n, s);
   }
 }
@@ -710,17 +742,19 @@ void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, t
   const int64_t chunks = (M + chunk - 1) / chunk;
   TORCH_CHECK(chunks * ntile < (int64_t(1) << 31), "linear_act: too many rows");
   torch::Tensor ws;
-  if (db) ws = torch::empty({chunks * N}, dy.options().dtype(torch::kFloat32));
+  const bool join = db && chunks > 1;
+  if (join) ws = torch::empty({chunks * N}, dy.options().dtype(torch::kFloat32));
   auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((unsigned)(chunks * ntile)), dim3(256), 0, stream,
                        (const T*)dy.data_ptr(), z ? (const T*)z->data_ptr() : nullptr,
-                       dz ? (T*)dz->data_ptr() : nullptr, db ? ws.data_ptr<float>() : nullptr, M, N, tile,
+                       dz ? (T*)dz->data_ptr() : nullptr, join ? ws.data_ptr<float>() : nullptr,
+                       db && !join ? (T*)db->data_ptr() : nullptr, M, N, tile,
                        ntile, (int)chunk, act);
   };
   if (vec) go(slope_kernel<T, V>);
   else go(slope_kernel<T, 1>);
-  if (db)
-    hipLaunchKernelGGL((column_join_kernel<T>), dim3((N + 31) / 32), dim3(1024), 0, stream,
+  if (join)
+    hipLaunchKernelGGL((column_join_kernel<T>), dim3((N + 7) / 8), dim3(1024), 0, stream,
                        ws.data_ptr<float>(), chunks, N, (T*)db->data_ptr());
 }
 

@@ -312,7 +312,7 @@ class FusedAdamW:
         self.step_count = zeros(1, torch.int64)
         self._lr_t = torch.full((1,), lr, device=dev, dtype=torch.float32)
         self._scal = zeros(3, torch.float32)
-        self._part = zeros(self._NORM_PARTS * 3, torch.float32)
+        self._part = zeros(self._NORM_PARTS * 3, torch.float64)
         self._seen = None       # addresses that the tables on the device were made for
         self._tables = None
 
@@ -402,8 +402,8 @@ class FusedAdamW:
             f = self.flat
             return (f.flat_param.data_ptr(), f.flat_grad.data_ptr(),
                     0 if f.flat_master is None else f.flat_master.data_ptr())
-        return [(p.data_ptr(), p.stride()) if p.grad is None else
-                (p.data_ptr(), p.stride(), p.grad.data_ptr(), p.grad.stride()) for p in self.params]
+        from .ops import ext
+        return ext().tensor_addresses(self.params)
 
     def _refresh_tables(self):
         """The device tables of addresses, made anew where an address changed."""
@@ -414,19 +414,28 @@ class FusedAdamW:
                                "keep them in place (zero_grad() fills them) and step once before capture")
         by = {}
         for kind, w, low, g, off, n, wd in self._views():
-            rows, chunks = by.setdefault(self._KINDS[kind], ([], []))
+            rows, lengths = by.setdefault(self._KINDS[kind], ([], []))
             pw, pl, pg = (0 if t is None else t.data_ptr() for t in (w, low, g))
             esize = kind.itemsize
             aligned = pw % 16 == 0 and off % 4 == 0 and pl % (4 * esize) == 0 and pg % (4 * esize) == 0
             bits = struct.unpack("<I", struct.pack("<f", wd))[0]
-            chunks += [(len(rows), i) for i in range(-(-n // self.CHUNK))]
             rows.append((pw, pl, pg, off, n, bits | (int(aligned) << 32)))
-        up = lambda v, t, c: torch.tensor(v, dtype=t).view(-1, c).pin_memory().to(self._dev, non_blocking=True)  # noqa: E731
+            lengths.append(-(-n // self.CHUNK))
+
+        def chunk_table(lengths):
+            """(row, chunk in the row) of every workgroup."""
+            count = torch.tensor(lengths)
+            row = torch.repeat_interleave(torch.arange(len(lengths)), count)
+            first = torch.cumsum(count, 0) - count
+            return torch.stack([row, torch.arange(row.numel()) - first[row]], 1).to(torch.int32)
+
+        up = lambda t: t.contiguous().pin_memory().to(self._dev, non_blocking=True)  # noqa: E731
+        rows = [up(torch.tensor(r, dtype=torch.int64).view(-1, 6)) for r, _ in by.values()]
+        chunks = [up(chunk_table(n)) for _, n in by.values()]
         if self._tables is not None:    # the old ones may still be read on this stream
             for t in self._tables[0] + self._tables[1]:
                 t.record_stream(torch.cuda.current_stream(self._dev))
-        self._tables = ([up(r, torch.int64, 6) for r, _ in by.values()],
-                        [up(c, torch.int32, 2) for _, c in by.values()], list(by))
+        self._tables = (rows, chunks, list(by))
         self._seen = self._addresses()
         return self._tables
 
