@@ -193,8 +193,9 @@ def run_epoch(model, loader, loss_fn, optimizer, desc_default="", epoch=0,
     graphed = None
     if (optimizer is not None and device != "cpu" and not use_mixup and not amp
             and os.environ.get("FAA_TRAIN_GRAPHS", "0") == "1"):
-        from ..optim import FusedRMSpropTF, FusedSGD
-        if isinstance(optimizer, (FusedSGD, FusedRMSpropTF)):
+        from ..optim import FusedAdamW, FusedRMSpropTF, FusedSGD
+        if (isinstance(optimizer, (FusedSGD, FusedRMSpropTF, FusedAdamW))
+                and optimizer.flat is not None):
             graphed = getattr(optimizer, "_faa_graph_step", None)
             if graphed is None:
                 graphed = _GraphedTrainStep(model, loss_fn, optimizer, flip_batch)
@@ -228,9 +229,10 @@ def run_epoch(model, loader, loss_fn, optimizer, desc_default="", epoch=0,
                 loss.backward()
                 if hasattr(model, "finish_gradient_sync"):
                     model.finish_gradient_sync()
-                from ..optim import FusedSGD, FusedRMSpropTF
-                if not isinstance(optimizer, (FusedSGD, FusedRMSpropTF)):
-                    # FusedSGD folds manual WD + global clip into its kernels
+                from ..optim import FusedAdamW, FusedSGD, FusedRMSpropTF
+                if not isinstance(optimizer, (FusedSGD, FusedRMSpropTF, FusedAdamW)):
+                    # FusedSGD folds manual WD + global clip into its kernels;
+                    # FusedAdamW clips there too, and its decay is decoupled
                     if wd > 0.0:
                         _apply_manual_wd(decay_params, wd)
                     grad_clip = conf["optimizer"].get("clip", 5.0)
@@ -303,13 +305,15 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
         device=device, out_dtype=out_dtype)
 
     # Fast path: pure-bf16 flat weights + fused optimizer + MFMA convs on GPU.
-    use_fast = (use_cuda and conf["optimizer"]["type"] in ("sgd", "rmsprop")
+    use_fast = (use_cuda and conf["optimizer"]["type"] in ("sgd", "rmsprop", "adamw")
                 and autocast_dtype == torch.bfloat16
                 and conf.get_value("pure_bf16", True))
     work_dtype = torch.bfloat16 if use_fast else None
 
+    # moments in 8 bits share a scale over 256 neighbours, which no two tensors should
+    flat_align = 256 if conf["optimizer"].get("state_bits", 32) == 8 else 64
     model = get_model(conf["model"], nc, local_rank=local_rank, device=device,
-                      work_dtype=work_dtype)
+                      work_dtype=work_dtype, flat_align=flat_align)
     model_ema = get_model(conf["model"], nc, local_rank=-1, device=device)
     model_ema.eval()
     if use_fast:
@@ -326,7 +330,7 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
         from ..optim import FusedSGD
         from ..parallel.flat import flatten_module
         flat = model.flat if hasattr(model, "flat") else \
-            flatten_module(model, work_dtype=torch.bfloat16)
+            flatten_module(model, align=flat_align, work_dtype=torch.bfloat16)
         patch_convs(model)
         if conf["optimizer"]["type"] == "sgd":
             optimizer = FusedSGD(flat, lr=conf["lr"],
@@ -334,6 +338,9 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
                                  nesterov=conf["optimizer"].get("nesterov", True),
                                  weight_decay=conf["optimizer"].get("decay", 0.0),
                                  grad_clip=conf["optimizer"].get("clip", 5.0))
+        elif conf["optimizer"]["type"] == "adamw":
+            from ..optim import build_adamw
+            optimizer = build_adamw(conf["optimizer"], flat, conf["lr"])
         else:
             from ..optim import FusedRMSpropTF
             optimizer = FusedRMSpropTF(flat, lr=conf["lr"], alpha=0.9,
@@ -341,6 +348,12 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
                                        weight_decay=conf["optimizer"].get("decay", 0.0),
                                        grad_clip=conf["optimizer"].get("clip", 0.0))
         autocast_dtype = None      # the model computes natively in bf16
+    elif conf["optimizer"]["type"] == "adamw":
+        decay = {id(p) for p in _decay_params(model)}
+        optimizer = build_optimizer(conf["optimizer"], [
+            {"params": [p for p in model.parameters() if id(p) in decay]},
+            {"params": [p for p in model.parameters() if id(p) not in decay], "weight_decay": 0.0},
+        ], conf["lr"])
     else:
         optimizer = build_optimizer(conf["optimizer"], model.parameters(), conf["lr"])
     scheduler = build_scheduler(conf.conf, optimizer, conf["lr"])

@@ -6,6 +6,8 @@ RCCL flat-buffer data-parallel engine instead of torch DDP.
 """
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import torch
 from torch import nn
@@ -19,7 +21,42 @@ from .efficientnet import EfficientNet, RoutingFn
 
 
 def build_model(conf, num_class: int = 10) -> nn.Module:
-    """Construct the bare module for a model conf dict (no device placement)."""
+    """Construct the bare module for a model conf dict (no device placement).
+
+    ``norm: group`` gives the architecture group norm for its BatchNorm
+    (``norm_groups`` of them, or their common divisor with the width), and puts
+    its linear layers on the fused products.
+    """
+    model = _build_architecture(conf, num_class)
+    norm = conf.get("norm", "batch")
+    if norm == "group":
+        from ..ops.pointwise import fuse_pointwise
+        model = to_group_norm(model, conf.get("norm_groups", 8))
+        fuse_pointwise(model)
+    elif norm != "batch":
+        raise NameError(f"no norm named {norm}")
+    return model
+
+
+def to_group_norm(model: nn.Module, groups: int = 8) -> nn.Module:
+    """Replace every BatchNorm2d by a group norm of gcd(groups, channels) groups with its weight and bias."""
+    from ..ops.groupnorm import GroupNormAct
+    if groups < 1:
+        raise ValueError(f"to_group_norm: groups={groups}")
+
+    def convert(m: nn.Module) -> nn.Module:
+        if isinstance(m, nn.BatchNorm2d):
+            gn = GroupNormAct(math.gcd(groups, m.num_features), m.num_features, eps=m.eps, affine=m.affine)
+            gn.weight, gn.bias = m.weight, m.bias
+            return gn
+        for name, child in m.named_children():
+            setattr(m, name, convert(child))
+        return m
+
+    return convert(model)
+
+
+def _build_architecture(conf, num_class: int) -> nn.Module:
     name = conf["type"]
     if name == "resnet50":
         return ResNet(dataset="imagenet", depth=50, num_classes=num_class, bottleneck=True)
@@ -72,7 +109,7 @@ def _tf_style_init(model: nn.Module) -> None:
 
 def get_model(conf, num_class: int = 10, local_rank: int = -1,
               device: str = "cuda", channels_last: bool = True,
-              work_dtype=None) -> nn.Module:
+              work_dtype=None, flat_align: int = 64) -> nn.Module:
     model = build_model(conf, num_class)
     name = conf["type"]
     if "efficientnet" in name and local_rank >= 0:
@@ -84,7 +121,7 @@ def get_model(conf, num_class: int = 10, local_rank: int = -1,
             model = model.to(memory_format=torch.channels_last)
     if local_rank >= 0:
         from ..parallel.ddp import FlatDDP
-        model = FlatDDP(model, work_dtype=work_dtype)
+        model = FlatDDP(model, work_dtype=work_dtype, align=flat_align)
     return model
 
 

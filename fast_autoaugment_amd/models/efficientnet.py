@@ -21,20 +21,21 @@ from torch.nn import functional as F
 
 from ..ops.functional import Swish, drop_connect
 from ..ops.modules import bn_only, bn_swish
+from ..ops.pointwise import linear_act
 
 
 def _bn(bn, x):
     """Fused BN kernel for plain BatchNorm2d (the 20%-of-step torch
     batch_norm_collect_statistics path in profiles/step_profile_efficientnet_b0_r01.txt);
     Tpu/Sync BN variants keep their own cross-replica forward."""
-    if type(bn) is nn.BatchNorm2d:
+    if type(bn) is nn.BatchNorm2d or isinstance(bn, nn.GroupNorm):
         return bn_only(x, bn)
     return bn(x)
 
 
 def _bn_swish(bn, x, swish_mod):
-    """BN + swish in one kernel for plain BatchNorm2d; composed otherwise."""
-    if type(bn) is nn.BatchNorm2d:
+    """BN + swish in one kernel for plain BatchNorm2d and GroupNorm; composed otherwise."""
+    if type(bn) is nn.BatchNorm2d or isinstance(bn, nn.GroupNorm):
         return bn_swish(x, bn)
     return swish_mod(bn(x))
 
@@ -202,6 +203,7 @@ class MBConvBlock(nn.Module):
         self._project_conv = make_conv(oup, block_args.output_filters, 1)
         self._bn2 = norm_layer(block_args.output_filters, momentum=bn_mom, eps=bn_eps)
         self._swish = Swish()
+        self.fused_se = False       # squeeze and excitation as two products with their activations
 
     def _is_condconv(self):
         return self.condconv_num_expert > 1
@@ -221,8 +223,13 @@ class MBConvBlock(nn.Module):
         x = _bn_swish(self._bn1, conv(self._depthwise_conv, x), self._swish)
         if self.has_se:
             sq = F.adaptive_avg_pool2d(x, 1)
-            sq = self._se_expand(self._swish(self._se_reduce(sq)))
-            x = torch.sigmoid(sq) * x
+            if self.fused_se and self._se_reduce.weight.dtype == sq.dtype:
+                gate = linear_act(sq.flatten(1), self._se_reduce.weight.flatten(1), self._se_reduce.bias, act="swish")
+                gate = linear_act(gate, self._se_expand.weight.flatten(1), self._se_expand.bias, act="sigmoid")
+                x = gate[:, :, None, None] * x
+            else:
+                sq = self._se_expand(self._swish(self._se_reduce(sq)))
+                x = torch.sigmoid(sq) * x
         x = _bn(self._bn2, conv(self._project_conv, x))
         if (self.id_skip and self._block_args.stride == 1
                 and self._block_args.input_filters == self._block_args.output_filters):

@@ -34,6 +34,8 @@ class WideBasic(nn.Module):
         if self.dropout.p > 0:
             out = self.dropout(out)
         out = self.conv2(bn_relu(out, self.bn2))
+        if isinstance(self.bn1, nn.GroupNorm):
+            return out + self.shortcut(x)       # no batch statistics to prepare
         return res_add(out, self.shortcut(x))
 
 

@@ -74,3 +74,12 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     if not x.is_cuda:
         return _composed(x, num_groups, weight, bias, eps, act)
     return require_ext_for(x).group_norm_act(x, num_groups, weight, bias, eps, ACTS[act])
+
+
+class GroupNormAct(torch.nn.GroupNorm):
+    """nn.GroupNorm on ``group_norm_act``; ``ops.modules`` fuses the activation that follows it."""
+
+    act = "none"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act)

@@ -5,6 +5,9 @@ on GPU it dispatches to the fused NHWC BatchNorm+ReLU HIP kernel
 (fwd + bwd as one custom Function); on CPU it composes torch ops. The BN
 module keeps standard nn.BatchNorm2d parameters/buffers so state_dicts stay
 checkpoint-compatible with the reference layout.
+
+A GroupNorm in the place of the BatchNorm (models built with ``norm: group``)
+goes to the fused group norm instead, on either device.
 """
 from __future__ import annotations
 
@@ -12,13 +15,20 @@ import torch
 import torch.nn.functional as F
 
 from . import has_ext
+from .groupnorm import group_norm_act
 
 
 import os
 
 
+def _group_norm(x: torch.Tensor, gn: torch.nn.GroupNorm, act: str) -> torch.Tensor:
+    return group_norm_act(x, gn.num_groups, gn.weight, gn.bias, gn.eps, act)
+
+
 def bn_relu(x: torch.Tensor, bn: torch.nn.BatchNorm2d) -> torch.Tensor:
     """BatchNorm2d followed by ReLU, fused on GPU."""
+    if isinstance(bn, torch.nn.GroupNorm):
+        return _group_norm(x, bn, "relu")
     if (x.is_cuda and has_ext()
             and os.environ.get("FAA_NO_FUSED_BN") != "1"):
         from .bnrelu import fused_bn_relu
@@ -28,6 +38,8 @@ def bn_relu(x: torch.Tensor, bn: torch.nn.BatchNorm2d) -> torch.Tensor:
 
 def bn_only(x: torch.Tensor, bn: torch.nn.BatchNorm2d) -> torch.Tensor:
     """BatchNorm2d without activation, fused on GPU."""
+    if isinstance(bn, torch.nn.GroupNorm):
+        return _group_norm(x, bn, "none")
     if (x.is_cuda and has_ext()
             and os.environ.get("FAA_NO_FUSED_BN") != "1"):
         from .bnrelu import fused_bn
@@ -37,6 +49,8 @@ def bn_only(x: torch.Tensor, bn: torch.nn.BatchNorm2d) -> torch.Tensor:
 
 def bn_swish(x: torch.Tensor, bn: torch.nn.BatchNorm2d) -> torch.Tensor:
     """BatchNorm2d followed by swish, fused on GPU (EfficientNet)."""
+    if isinstance(bn, torch.nn.GroupNorm):
+        return _group_norm(x, bn, "swish")
     if (x.is_cuda and has_ext()
             and os.environ.get("FAA_NO_FUSED_BN") != "1"):
         from .bnrelu import fused_bn_swish

@@ -81,3 +81,27 @@ def conv1x1_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         weight = weight.flatten(1)
     last = lambda t: None if t is None else t.permute(0, 2, 3, 1)  # noqa: E731
     return linear_act(last(x), weight, bias, last(residual), act).permute(0, 3, 1, 2)
+
+
+class LinearAct(torch.nn.Linear):
+    """nn.Linear on ``linear_act`` where x has the weights' type (under autocast it may not: torch's product then)."""
+
+    act = "none"
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dtype != self.weight.dtype or x.dtype not in _DTYPES:
+            return torch.nn.functional.linear(x, self.weight, self.bias)
+        return linear_act(x, self.weight, self.bias, act=self.act)
+
+
+def fuse_pointwise(model: torch.nn.Module) -> int:
+    """Put a model's linear heads and squeeze-and-excitation products on ``linear_act``. Returns how many."""
+    n = 0
+    for m in model.modules():
+        if type(m) is torch.nn.Linear:
+            m.__class__ = LinearAct
+            n += 1
+        elif getattr(m, "has_se", False) and hasattr(m, "fused_se"):
+            m.fused_se = True
+            n += 2
+    return n

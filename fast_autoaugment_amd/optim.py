@@ -171,7 +171,16 @@ def build_optimizer(conf_opt, model_params, lr: float):
     if typ == "rmsprop":
         return RMSpropTF(model_params, lr=lr, weight_decay=0.0,
                          alpha=0.9, momentum=0.9, eps=0.001)
+    if typ == "adamw":
+        return build_adamw(conf_opt, model_params, lr)
     raise ValueError(f"invalid optimizer type={typ}")
+
+
+def build_adamw(conf_opt, params, lr: float):
+    """FusedAdamW from a conf['optimizer'] dict: decay (decoupled), betas, eps, clip and state_bits (8 or 32)."""
+    return FusedAdamW(params, lr=lr, betas=tuple(conf_opt.get("betas", (0.9, 0.999))),
+                      eps=float(conf_opt.get("eps", 1e-8)), weight_decay=conf_opt.get("decay", 0.0),
+                      grad_clip=conf_opt.get("clip", 5.0), state_bits=conf_opt.get("state_bits", 32))
 
 
 class FusedRMSpropTF:

@@ -30,7 +30,9 @@ _MODEL_CACHE: Dict = {}
 
 def _cached_model(conf, nc, save_path: str, device: str):
     import os as _os
-    key = (save_path, conf["model"].get("type"), nc)
+    # fold_inference: the frozen child's 1x1 convolutions with their BatchNorm, skip and activation as one product
+    fold = bool(conf.get_value("fold_inference", False))
+    key = (save_path, conf["model"].get("type"), nc, fold)
     mtime = _os.path.getmtime(save_path)
     hit = _MODEL_CACHE.get(key)
     if hit is not None and hit[0] == mtime:
@@ -40,6 +42,10 @@ def _cached_model(conf, nc, save_path: str, device: str):
     sd = ckpt["model"] if "model" in ckpt else ckpt
     model.load_state_dict({k.replace("module.", ""): v for k, v in sd.items()})
     model.eval()
+    if fold:
+        from ..models.folded import fold_for_inference
+        bf16 = device != "cpu" and conf.get_value("precision", "bf16") == "bf16"
+        fold_for_inference(model, torch.bfloat16 if bf16 else torch.float32)
     _MODEL_CACHE.clear()
     _MODEL_CACHE[key] = (mtime, model)
     return model
