@@ -425,6 +425,78 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
   }
 }
 
+// Few outputs: 32 x 32 of them a workgroup, and its 4 waves take every fourth step of k each, with buffers of their
+// own and no barrier between them; their sums meet in LDS at the end. One launch where the large tiles would have
+// to be split over workgroups and joined.
+template <typename T, bool PR, bool QR>
+__global__ __launch_bounds__(256) void small_product_kernel(Operand P, Operand Q, Epilogue<T> epi, int tiles_n) {
+  constexpr int B = 32;
+  typedef Loader<B, PR, false, 64> LP;
+  typedef Loader<B, QR, true, 64> LQ;
+  __shared__ __align__(16) short p0[4][B * BK], p1[4][B * BK], q0[4][B * BK], q1[4][B * BK];
+  const uint32_t tm = blockIdx.x / (uint32_t)tiles_n;
+  const int m0 = (int)tm * B, n0 = (int)(blockIdx.x - tm * tiles_n) * B;
+  const int steps = (P.kdim + BK - 1) / BK;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LP load_p(P, m0, lane);
+  const LQ load_q(Q, n0, lane);
+  f32x4 acc[2][2];
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0, 0, 0, 0};
+  auto fill = [&](int s, short* p, short* q) {
+    load_p(s * BK, s < steps, p, 0);
+    load_q(s * BK, s < steps, q, 0);
+  };
+  // the older of two steps' pieces have come (see product_kernel); fragments are read, and may be overwritten
+  auto come = [] { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(LP::N + LQ::N) : "memory"); };
+  auto read = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+  auto multiply = [&](const short* p, const short* q) {
+    #pragma unroll
+    for (int k = 0; k < BK; k += 32) {
+      s16x8 fp[2], fq[2];
+      #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fp[i] = LP::L::fragment(p, 0, i, k, lane);
+        fq[i] = LQ::L::fragment(q, 0, i, k, lane);
+      }
+      #pragma unroll
+      for (int i = 0; i < 2; ++i)
+        #pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
+    }
+  };
+  fill(wave, p0[wave], q0[wave]);
+  fill(wave + 4, p1[wave], q1[wave]);
+  for (int s = wave; s < steps; s += 8) {
+    come();
+    multiply(p0[wave], q0[wave]);
+    read();
+    fill(s + 8, p0[wave], q0[wave]);
+    come();
+    multiply(p1[wave], q1[wave]);       // zeros where the step is not there
+    read();
+    fill(s + 12, p1[wave], q1[wave]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  // the waves' sums, 32 lines of 32 and 4 more (a line's start moves by 4 banks)
+  constexpr int LD = B + 4;
+  __shared__ __align__(16) float sums[4 * B * LD];
+  #pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float* line = sums + (wave * B + i * 16 + (lane & 15)) * LD + (lane >> 4) * 8;
+    *(f32x4*)line = acc[i][0];
+    *(f32x4*)(line + 4) = acc[i][1];
+  }
+  __syncthreads();
+  const int row = tid >> 3, col = (tid & 7) * 4, N = Q.rows;
+  f32x4 v = {0, 0, 0, 0};
+  #pragma unroll
+  for (int w = 0; w < 4; ++w) v += *(const f32x4*)(sums + (w * B + row) * LD + col);
+  if (m0 + row < P.rows)
+    by_act<!PR && !QR>(epi.act, [&](auto A) { epi.template four<A.value>(m0 + row, n0 + col, N, v); });
+}
+
 // lines of `from` values into lines of `to`, a multiple of 8, with zeros behind
 __global__ __launch_bounds__(256) void widen_lines_kernel(const short* __restrict__ in, short* __restrict__ out,
                                                           int64_t lines, int from, int to) {
@@ -695,10 +767,23 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
     if (BM == 128 && N > 64 && (tiles(128, 128) >= 256 || K >= 8192)) BN = 128;
   }
   const int64_t tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, steps = (K + step - 1) / step;
-  // few tiles and a long k: enough parts for 2 workgroups a CU, each with 4 steps at least
+  // few tiles and a long k: parts for one workgroup a CU, each with 4 steps at least. More parts are more fp32 to
+  // write and read again: dW of 25088x1024x256 takes 25 us with 256 workgroups, 27 with 512, 38 with 1024.
   int64_t splits = 1;
-  if (tm * tn < 256) splits = std::max<int64_t>(1, std::min<int64_t>(512 / (tm * tn), steps / 4));
+  if (tm * tn < 256) splits = std::max<int64_t>(1, std::min<int64_t>(256 / (tm * tn), steps / 4));
   TORCH_CHECK(tm * tn * splits < (int64_t(1) << 31), "linear_act: too many tiles");
+  if constexpr (sizeof(T) == 2) {
+    // Measured (us, this/large tiles): 128x1152x48 4.5/6.4, 100x1280x1000 4.8/7.5, 512x1280x1000 (512 tiles) 8.7/10.1;
+    // but 2048x1280x1000 (2048 tiles) 31/12, k = 6272 for 128x512 17/10, and k = 320 for 512x1280 (640) 7.8/3.9.
+    const int64_t sm = (M + 31) / 32, sn = (N + 31) / 32;
+    if (tm * tn < 256 && sm * sn <= 512 && steps >= 4 && steps <= 40) {
+      torch::Tensor keep_p, keep_q;
+      const Operand P = operand(p, PR, keep_p, stream), Q = operand(q, QR, keep_q, stream);
+      hipLaunchKernelGGL((small_product_kernel<T, PR, QR>), dim3((unsigned)(sm * sn)), dim3(256), 0, stream, P, Q,
+                         epi, (int)sn);
+      return;
+    }
+  }
   torch::Tensor ws;
   float* part = nullptr;
   if (splits > 1) {
@@ -736,8 +821,8 @@ void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, t
                    && aligned(z->data_ptr(), 16)));
   const int vw = vec ? V : 1, tile = std::min(N, (vec ? 32 : 64) * vw), ntile = (N + tile - 1) / tile;
   const int rows = 256 / (tile / vw);
-  // about 2048 workgroups, and chunks of 8 rows a thread at least
-  int64_t chunk = std::max<int64_t>(8, (M * ntile / 2048 + rows - 1) / rows) * rows;
+  // about 2048 workgroups, and chunks of 16 rows a thread at least
+  int64_t chunk = std::max<int64_t>(16, (M * ntile / 2048 + rows - 1) / rows) * rows;
   chunk = std::min<int64_t>(chunk, 1 << 24);
   const int64_t chunks = (M + chunk - 1) / chunk;
   TORCH_CHECK(chunks * ntile < (int64_t(1) << 31), "linear_act: too many rows");
