@@ -769,26 +769,33 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
   });
 }
 
-// dw[c], db[c]: the sums over n rows of ws[row][{sum dz, sum dz xhat}][C], 32 columns a workgroup
+// out[y][column] = sum over the rows y*per .. of ws[row][2C], 32 columns a workgroup; where there is one y, the
+// columns are db (sum dz) and dw (sum dz xhat)
 template <typename W>
 __global__ __launch_bounds__(1024) void gn_param_grads_kernel(const float* __restrict__ ws, int64_t n,
-                                                              int C, W* __restrict__ dw,
-                                                              W* __restrict__ db) {
+                                                              int64_t per, int C, float* __restrict__ out,
+                                                              W* __restrict__ dw, W* __restrict__ db) {
   __shared__ float lds[32][33];
   const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
   const int64_t i = (int64_t)blockIdx.x * 32 + col;       // of the 2C columns
+  const int64_t r0 = blockIdx.y * per, r1 = min(r0 + per, n);
   float s = 0.0f;
   if (i < 2 * (int64_t)C)
-    for (int64_t r = row; r < n; r += 32) s += ws[r * 2 * C + i];
+    #pragma unroll 4
+    for (int64_t r = r0 + row; r < r1; r += 32) s += ws[r * 2 * C + i];
   lds[row][col] = s;
   __syncthreads();
   if (row == 0 && i < 2 * (int64_t)C) {
     s = 0.0f;
     #pragma unroll
     for (int r = 0; r < 32; ++r) s += lds[r][col];
-    W* out = i < C ? db + i : dw + (i - C);
-    if constexpr (sizeof(W) == 4) *(float*)out = s;
-    else *(unsigned short*)out = float_to_bits<W>(s);
+    if (out) {
+      out[blockIdx.y * 2 * (int64_t)C + i] = s;
+      return;
+    }
+    W* to = i < C ? db + i : dw + (i - C);
+    if constexpr (sizeof(W) == 4) *(float*)to = s;
+    else *(unsigned short*)to = float_to_bits<W>(s);
   }
 }
 
@@ -847,7 +854,8 @@ Chunks chunks_of(const Shape& s, int R) {
   c.chunk = rows * R;
   c.nchunk = (s.S + c.chunk - 1) / c.chunk;
   c.wgs = s.B * c.ntile * c.nchunk;
-  TORCH_CHECK(c.wgs < (int64_t(1) << 31) && s.B * s.G < (int64_t(1) << 31), "group_norm: too large");
+  TORCH_CHECK(c.wgs < (int64_t(1) << 24) && s.B * s.G < (int64_t(1) << 24),
+              "group_norm_act: more workgroups than a launch takes");     // 2^32 threads
   return c;
 }
 
@@ -886,7 +894,7 @@ bool whole_of(const Shape& s, Whole& out) {
   }
   out.tile = (int)(k * unit);
   out.ntile = (int)((units + k - 1) / k);
-  if (workgroups(k) >= (int64_t(1) << 31)) return false;
+  if (workgroups(k) >= (int64_t(1) << 22)) return false;
   for (int threads : {256, 512, 1024})
     for (out.r = 1; out.r <= MOST_R; out.r *= 2) {
       out.threads = (int)((((int64_t)s.S + out.r - 1) / out.r * (out.tile / VEC) + 63) / 64 * 64);
@@ -1057,8 +1065,19 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
         if (nw || nb)
           by_type(dw.scalar_type(), [&](auto z) {
             using W = decltype(z);
-            hipLaunchKernelGGL((gn_param_grads_kernel<W>), dim3((2 * s.C + 31) / 32), dim3(1024), 0, stream,
-                               sums.data_ptr<float>(), sums.size(0), s.C, (W*)dw.data_ptr(),
+            const unsigned columns = (unsigned)((2 * (int64_t)s.C + 31) / 32);
+            int64_t n = sums.size(0);
+            if (n > 2048) {       // many small samples: 1024 of them a workgroup first
+              const int64_t per = std::max<int64_t>(1024, (n + 32767) / 32768), parts = (n + per - 1) / per;
+              auto joined = torch::empty({parts, 2 * (int64_t)s.C}, sums.options());
+              hipLaunchKernelGGL((gn_param_grads_kernel<W>), dim3(columns, (unsigned)parts), dim3(1024), 0,
+                                 stream, sums.data_ptr<float>(), n, per, s.C, joined.data_ptr<float>(),
+                                 (W*)nullptr, (W*)nullptr);
+              sums = joined;
+              n = parts;
+            }
+            hipLaunchKernelGGL((gn_param_grads_kernel<W>), dim3(columns), dim3(1024), 0, stream,
+                               sums.data_ptr<float>(), n, n, s.C, (float*)nullptr, (W*)dw.data_ptr(),
                                (W*)db.data_ptr());
           });
         C10_HIP_KERNEL_LAUNCH_CHECK();

@@ -123,7 +123,7 @@ __device__ __forceinline__ float act_value(float z) {
   if (ACT == ACT_SIGMOID) return sigmoid(z);
   return z;
 }
-// from z, or for relu from y: both are above 0 in the same places
+// from z, or for relu from y: both are above 0 in the same places, but for z below half the type's smallest number
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
@@ -771,7 +771,7 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
   // write and read again: dW of 25088x1024x256 takes 25 us with 256 workgroups, 27 with 512, 38 with 1024.
   int64_t splits = 1;
   if (tm * tn < 256) splits = std::max<int64_t>(1, std::min<int64_t>(256 / (tm * tn), steps / 4));
-  TORCH_CHECK(tm * tn * splits < (int64_t(1) << 31), "linear_act: too many tiles");
+  TORCH_CHECK(tm * tn * splits < (int64_t(1) << 24), "linear_act: too many tiles");     // 2^32 threads a launch
   if constexpr (sizeof(T) == 2) {
     // Measured (us, this/large tiles): 128x1152x48 4.5/6.4, 100x1280x1000 4.8/7.5, 512x1280x1000 (512 tiles) 8.7/10.1;
     // but 2048x1280x1000 (2048 tiles) 31/12, k = 6272 for 128x512 17/10, and k = 320 for 512x1280 (640) 7.8/3.9.
@@ -825,7 +825,7 @@ void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, t
   int64_t chunk = std::max<int64_t>(16, (M * ntile / 2048 + rows - 1) / rows) * rows;
   chunk = std::min<int64_t>(chunk, 1 << 24);
   const int64_t chunks = (M + chunk - 1) / chunk;
-  TORCH_CHECK(chunks * ntile < (int64_t(1) << 31), "linear_act: too many rows");
+  TORCH_CHECK(chunks * ntile < (int64_t(1) << 24), "linear_act: too many rows");
   torch::Tensor ws;
   const bool join = db && chunks > 1;
   if (join) ws = torch::empty({chunks * N}, dy.options().dtype(torch::kFloat32));

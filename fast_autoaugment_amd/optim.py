@@ -274,8 +274,8 @@ class FusedAdamW:
     ``exp_avg_root``) with one fp32 scale for every 256 neighbours of a tensor
     (``*_scale``); the step uses the moments before they are rounded. A flat
     buffer then has to start each tensor at a multiple of 256
-    (``flatten_module(align=256)``). A block with a NaN or an infinity in it is
-    no number as a whole from then on.
+    (``flatten_module(align=256)``). A NaN stays in its element; an infinite
+    moment makes its block of 256 NaN from the next step on.
 
     The step count and the learning rate are on the device: a captured step
     replays, with ``sync_lr()`` before a replay pushing a changed rate. Under
@@ -324,6 +324,7 @@ class FusedAdamW:
         self._part = zeros(self._NORM_PARTS * 3, torch.float64)
         self._seen = None       # addresses that the tables on the device were made for
         self._tables = None
+        self._captured = []
 
     # ---- what there is to update: (weights fp32, low-precision copy, gradient's owner, offset, n, decay)
 
@@ -416,9 +417,12 @@ class FusedAdamW:
 
     def _refresh_tables(self):
         """The device tables of addresses, made anew where an address changed."""
+        capturing = torch.cuda.is_current_stream_capturing()
         if self._addresses() == self._seen:
+            if capturing and not any(t is self._tables for t in self._captured):
+                self._captured.append(self._tables)     # a graph reads them as long as it is replayed
             return self._tables
-        if torch.cuda.is_current_stream_capturing():
+        if capturing:
             raise RuntimeError("FusedAdamW: the gradients' addresses changed since the last eager step: "
                                "keep them in place (zero_grad() fills them) and step once before capture")
         by = {}
@@ -543,6 +547,8 @@ class FusedAdamW:
 
     @torch.no_grad()
     def load_state_dict(self, sd):
+        if "exp_avg" not in sd or "step" not in sd:
+            raise ValueError("FusedAdamW: this is not the state of a FusedAdamW")
         bits = 32 if "exp_avg_sq" in sd else 8
         if bits != self.state_bits:
             raise ValueError(f"FusedAdamW: the state is held in {bits} bits, this optimizer's in {self.state_bits}")

@@ -222,6 +222,11 @@ def test_refusals():
         opt.load_state_dict(FusedAdamW([p()], state_bits=8).state_dict())
     with pytest.raises(ValueError):
         opt.load_state_dict(FusedAdamW([p(300)]).state_dict())
+    with pytest.raises(ValueError):
+        opt.load_state_dict({"momentum_buf": torch.zeros(3)})
+    q.grad = torch.zeros(3).to_sparse()
+    with pytest.raises(TypeError):
+        opt.step()
     strided = nn.Parameter(torch.zeros(4, 6)[:, ::2])
     strided.grad = torch.zeros(4, 3)
     with pytest.raises(ValueError):
@@ -293,6 +298,48 @@ def test_captured_steps_follow_eager_ones(bits):
     with pytest.raises(RuntimeError):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             opt_a.step()
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    p = nn.Parameter(torch.zeros(300, device="cuda"))
+    p.grad = torch.ones(300, device="cuda")
+    opt = FusedAdamW([p])
+    opt.step()
+    p.grad = torch.ones(300, device="cuda").to_sparse()
+    with pytest.raises(TypeError):
+        opt.step()
+    p.grad = torch.ones(300, device="cuda")
+    p.data = torch.zeros(200, device="cuda")
+    p.grad = torch.ones(200, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step()
+    with pytest.raises(ValueError):
+        FusedAdamW([nn.Parameter(torch.zeros(3, device="cuda")), nn.Parameter(torch.zeros(3))])
+
+
+@pytest.mark.gpu
+def test_a_captured_step_outlives_new_gradients():
+    """A graph keeps the tables it was captured with, whatever eager steps on other gradients make later."""
+    p = nn.Parameter(torch.zeros(5000, device="cuda"))
+    first = p.grad = torch.ones(5000, device="cuda")
+    opt = FusedAdamW([p], lr=1e-2)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    held = []
+    for i in range(4):
+        p.grad = torch.full((5000,), float(i), device="cuda")
+        opt.step()
+        held.append(torch.full((64,), -1, dtype=torch.int64, device="cuda"))      # where old tables may have been
+    torch.cuda.synchronize()
+    first.fill_(1.0)
+    before, moment = p.detach().clone(), opt.exp_avg.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    want = 0.9 * moment[:5000] + 0.1 * first
+    assert torch.allclose(opt.exp_avg[:5000], want, rtol=2.0 ** -22) and not torch.equal(before, p.detach())
 
 
 @pytest.mark.gpu

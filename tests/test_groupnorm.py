@@ -89,7 +89,8 @@ SHAPES = [
     ((1, 16, 130, 130), 4), ((2, 8, 2, 3, 4), 2), ((4, 2048, 2, 2), 1), ((2, 2047, 2, 1), 1),
     ((5, 32, 32, 32), 32), ((1, 16, 1, 1), 1), ((3, 40, 56, 56), 5), ((2, 256, 56, 56), 32),
     ((300, 16, 2, 2), 2), ((2, 672, 14, 14), 8), ((1, 96, 112, 112), 8), ((2, 4096, 1, 1), 2),
-    ((1, 20, 64, 64), 1), ((9, 192, 8, 8), 3),
+    ((1, 20, 64, 64), 1), ((9, 192, 8, 8), 3), ((5000, 24), 3), ((2, 28, 13, 11), 7), ((2, 36, 90, 90), 2),
+    ((128, 16, 56, 56), 8), ((3, 1000, 5, 5), 8), ((2, 1024, 16, 16), 1),
 ]
 
 
