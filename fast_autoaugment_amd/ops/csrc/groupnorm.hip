@@ -806,13 +806,21 @@ struct Shape {
   int S, C, G, cg;
 };
 
-// x: [N, ..., C], contiguous
+// t with its channels last in memory, whatever its order is: [N, C, ...] over lines of C
+torch::Tensor channels_last(const torch::Tensor& t) {
+  if (t.dim() == 4) return t.contiguous(at::MemoryFormat::ChannelsLast);
+  if (t.dim() == 5) return t.contiguous(at::MemoryFormat::ChannelsLast3d);
+  if (t.dim() == 2) return t.contiguous();
+  return t.movedim(1, -1).contiguous().movedim(-1, 1);
+}
+
+// x: [N, C, ...], channels last
 Shape shape_of(const torch::Tensor& x, int64_t groups, const torch::Tensor& w, const torch::Tensor& b,
                int64_t act) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.dim() >= 2, "group_norm_act: [N, C, ...] on the GPU");
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 2, "group_norm_act: [N, C, ...] on the GPU");
   Shape s;
   s.B = x.size(0);
-  const int64_t C = x.size(-1), S = x.numel() ? x.numel() / (s.B * C) : 0;
+  const int64_t C = x.size(1), S = x.numel() ? x.numel() / (s.B * C) : 0;
   TORCH_CHECK(S * C < (int64_t(1) << 31), "group_norm_act: a sample has 2^31 values or more");
   TORCH_CHECK(C < (1 << 23), "group_norm_act: 2^23 channels or more");
   TORCH_CHECK(groups > 0 && C > 0 && C % groups == 0, "group_norm_act: C is no multiple of the groups");
@@ -1005,10 +1013,10 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
                                c10::optional<torch::Tensor> weight, c10::optional<torch::Tensor> bias,
                                double eps, int64_t act) {
     const c10::OptionalDeviceGuard guard(x.device());
-    auto rows = x.movedim(1, -1).contiguous();
+    auto rows = channels_last(x);
     auto w = weight ? weight->contiguous() : torch::Tensor(), b = bias ? bias->contiguous() : torch::Tensor();
     const Shape s = shape_of(rows, groups, w, b, act);
-    auto y = at::empty_strided(x.sizes(), rows.movedim(-1, 1).strides(), x.options());
+    auto y = at::empty_strided(rows.sizes(), rows.strides(), rows.options());
     auto stat = x.options().dtype(torch::kFloat32);
     auto mean = torch::empty({s.B, s.G}, stat), rstd = torch::empty({s.B, s.G}, stat);
     if (x.numel() > 0) {
@@ -1021,8 +1029,7 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
       });
     }
     C10_HIP_KERNEL_LAUNCH_CHECK();
-    ctx->saved_data["groups"] = groups;
-    ctx->saved_data["act"] = act;
+    ctx->saved_data["how"] = groups * 4 + act;
     ctx->save_for_backward({rows, w, b, mean, rstd});
     return y;
   }
@@ -1032,7 +1039,8 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
     const bool again = at::GradMode::is_enabled();
     auto saved = ctx->get_saved_variables();
     const auto &x = saved[0], &w = saved[1], &b = saved[2], &mean = saved[3], &rstd = saved[4];
-    const int act = (int)ctx->saved_data["act"].toInt();
+    const int64_t how = ctx->saved_data["how"].toInt();
+    const int act = (int)(how % 4);
     const c10::OptionalDeviceGuard guard(x.device());
     auto stream = at::hip::getCurrentHIPStream().stream();
     // absent tensors are not counted among the inputs
@@ -1041,9 +1049,9 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
     torch::Tensor dx, dw, db;
     {
       at::NoGradGuard off;
-      const Shape s = shape_of(x, ctx->saved_data["groups"].toInt(), w, b, act);
-      auto dy = grads[0].movedim(1, -1).contiguous();
-      dx = torch::empty_like(x);
+      const Shape s = shape_of(x, how / 4, w, b, act);
+      auto dy = channels_last(grads[0]);
+      dx = at::empty_strided(x.sizes(), x.strides(), x.options());
       auto popt = (w.defined() ? w : b.defined() ? b : mean).options();
       if (nw || nb) {
         dw = torch::empty({s.C}, popt);
@@ -1083,7 +1091,7 @@ class GroupNormAct : public torch::autograd::Function<GroupNormAct> {
         C10_HIP_KERNEL_LAUNCH_CHECK();
       }
     }
-    torch::autograd::variable_list out{dx.movedim(-1, 1), torch::Tensor(), nw ? dw : torch::Tensor(),
+    torch::autograd::variable_list out{dx, torch::Tensor(), nw ? dw : torch::Tensor(),
                                        nb ? db : torch::Tensor(), torch::Tensor(), torch::Tensor()};
     if (again)      // differentiating these again is an error, not a zero
       for (auto& g : out)

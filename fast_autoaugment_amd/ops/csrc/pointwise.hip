@@ -881,9 +881,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
         product<T, false, false>(x, w, epi, stream);
       });
     C10_HIP_KERNEL_LAUNCH_CHECK();
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["bias"] = b.defined();
-    ctx->saved_data["res"] = r.defined();
+    ctx->saved_data["how"] = act * 4 + b.defined() * 2 + r.defined();
     // relu's slope is known from its result
     ctx->save_for_backward({x, w, keep ? z : act == ACT_RELU ? y : torch::Tensor()});
     return y;
@@ -893,11 +891,12 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
                                                  torch::autograd::variable_list grads) {
     auto saved = ctx->get_saved_variables();
     const auto &x = saved[0], &w = saved[1], &z = saved[2];
-    const int act = (int)ctx->saved_data["act"].toInt();
+    const int64_t how = ctx->saved_data["how"].toInt();
+    const int act = (int)(how / 4);
     const c10::OptionalDeviceGuard guard(x.device());
     auto stream = at::hip::getCurrentHIPStream().stream();
     // absent tensors are not counted among the inputs
-    const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["res"].toBool();
+    const bool has_b = how & 2, has_r = how & 1;
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1),
                nb = has_b && ctx->needs_input_grad(2), nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
     torch::Tensor dy, dz, dx, dw, db;
