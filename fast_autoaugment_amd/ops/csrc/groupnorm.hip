@@ -320,36 +320,84 @@ __global__ __launch_bounds__(256) void gn_chunk_stats_kernel(
   }
 }
 
-// one workgroup a group: its mean, and the parts' squares moved to it
+// Joins: a workgroup has `gt` groups of a sample, so that lines of the chunks' sums are read whole. Threads lie as
+// parts x channels; what they leave in LDS is added a channel, then a group (a wave each).
+struct Join {
+  int64_t b;
+  int g0, groups, ch, parts, part, col;
+  __device__ __forceinline__ Join(int G, int cg, int gt) {
+    const uint32_t tiles = (G + gt - 1) / gt, bi = blockIdx.x / tiles;
+    b = bi;
+    g0 = (int)(blockIdx.x - bi * tiles) * gt;
+    groups = min(gt, G - g0);
+    ch = groups * cg;
+    parts = max(1, 256 / ch);
+    part = (int)threadIdx.x / ch;
+    col = (int)threadIdx.x - part * ch;
+    if (ch > 256) { part = 0; col = threadIdx.x; }
+  }
+};
+
+// mean and rstd of every group from the chunks' means and squares, which are moved to the joined means
 __global__ __launch_bounds__(256) void gn_join_stats_kernel(
     const float* __restrict__ ws, float* __restrict__ mean_out, float* __restrict__ rstd_out, int S,
-    int C, int cg, int nchunk, int chunk, float eps) {
-  __shared__ float lds[4];
-  const uint32_t G = C / cg, bi = blockIdx.x / G;
-  const int g = (int)(blockIdx.x - bi * G);
-  const int64_t b = bi;
-  const float* p = ws + b * nchunk * 2 * C + g * cg;
-  float s = 0.0f;
-  for (int i = threadIdx.x; i < cg * nchunk; i += blockDim.x) {
-    const int k = i / cg, c = i - k * cg;
-    s += p[(int64_t)k * 2 * C + c] * min(chunk, S - k * chunk);
+    int C, int cg, int gt, int nchunk, int chunk, float eps) {
+  extern __shared__ float lds[];                // {mean, m2} x channels, then {n, mean, m2} x threads
+  const int G = C / cg;
+  const Join j(G, cg, gt);
+  const float* p = ws + j.b * nchunk * 2 * C + j.g0 * cg;
+  float* share = lds + 2 * j.ch;
+  for (int c0 = 0; c0 < j.ch; c0 += 256) {
+    const int c = c0 + j.col;
+    float s = 0.0f, n = 0.0f, q = 0.0f, m = 0.0f;
+    const bool on = j.part < j.parts && c < j.ch;
+    if (on) {
+      #pragma unroll 4
+      for (int k = j.part; k < nchunk; k += j.parts) {
+        const float np = (float)min(chunk, S - k * chunk);
+        s += p[(int64_t)k * 2 * C + c] * np;
+        n += np;
+      }
+      m = n > 0.0f ? s / n : 0.0f;
+      #pragma unroll 4
+      for (int k = j.part; k < nchunk; k += j.parts) {
+        const float d = p[(int64_t)k * 2 * C + c] - m;
+        q += p[(int64_t)k * 2 * C + C + c] + d * d * (float)min(chunk, S - k * chunk);
+      }
+    }
+    __syncthreads();
+    share[threadIdx.x] = n;
+    share[256 + threadIdx.x] = m;
+    share[512 + threadIdx.x] = q;
+    __syncthreads();
+    if (on && j.part == 0) {
+      float sum = 0.0f;
+      for (int k = 0; k < j.parts; ++k) sum += share[k * j.ch + j.col] * share[256 + k * j.ch + j.col];
+      const float mean = sum / (float)S;
+      float m2 = 0.0f;
+      for (int k = 0; k < j.parts; ++k) {
+        const float d = share[256 + k * j.ch + j.col] - mean;
+        m2 += share[512 + k * j.ch + j.col] + share[k * j.ch + j.col] * d * d;
+      }
+      lds[c] = mean;
+      lds[j.ch + c] = m2;
+    }
   }
-  s = faa_block_reduce_sum(s, lds);
-  __shared__ float mean_s;
-  const float count = (float)cg * (float)S;
-  if (threadIdx.x == 0) mean_s = s / count;
   __syncthreads();
-  const float mean = mean_s;
-  s = 0.0f;
-  for (int i = threadIdx.x; i < cg * nchunk; i += blockDim.x) {
-    const int k = i / cg, c = i - k * cg;
-    const float d = p[(int64_t)k * 2 * C + c] - mean;
-    s += p[(int64_t)k * 2 * C + C + c] + d * d * min(chunk, S - k * chunk);
-  }
-  s = faa_block_reduce_sum(s, lds);
-  if (threadIdx.x == 0) {
-    mean_out[blockIdx.x] = mean;
-    rstd_out[blockIdx.x] = 1.0f / sqrtf(s / count + eps);
+  const int lane = threadIdx.x & 63;
+  for (int g = (int)threadIdx.x >> 6; g < j.groups; g += 4) {
+    float s = 0.0f, q = 0.0f;
+    for (int c = lane; c < cg; c += 64) s += lds[g * cg + c];
+    const float mean = wave_sum(s) / (float)cg;
+    for (int c = lane; c < cg; c += 64) {
+      const float d = lds[g * cg + c] - mean;
+      q += lds[j.ch + g * cg + c] + (float)S * d * d;
+    }
+    const float rstd = 1.0f / sqrtf(wave_sum(q) / ((float)cg * (float)S) + eps);
+    if (lane == 0) {
+      mean_out[j.b * G + j.g0 + g] = mean;
+      rstd_out[j.b * G + j.g0 + g] = rstd;
+    }
   }
 }
 
@@ -489,52 +537,60 @@ __global__ __launch_bounds__(256) void gn_chunk_grads_kernel(
   }
 }
 
-// one workgroup a group: means[sample][group] = {mean u, mean u xhat}, and the chunks' sums joined a channel
-// to sample[sample][{sum dz, sum dz xhat}][C], which the parameters' gradients are made of
+// means[sample][group] = {mean u, mean u xhat}, and the chunks' sums joined a channel to
+// sample[sample][{sum dz, sum dz xhat}][C], which the parameters' gradients are made of
 template <typename T>
 __global__ __launch_bounds__(256) void gn_join_grads_kernel(
     const float* __restrict__ ws, const void* __restrict__ w, bool f32, float* __restrict__ means,
-    float* __restrict__ sample, int S, int C, int cg, int nchunk) {
-  __shared__ float lds[2][256];
-  __shared__ float red[4];
-  const uint32_t G = C / cg, bi = blockIdx.x / G;
-  const int g = (int)(blockIdx.x - bi * G);
-  const int64_t b = bi;
-  const float* p = ws + b * nchunk * 2 * C + g * cg;
-  const int wide = min(cg, 256), parts = 256 / wide, part = (int)threadIdx.x / wide,
-            col = (int)threadIdx.x - part * wide;
-  float s1 = 0.0f, s2 = 0.0f;
-  for (int c0 = 0; c0 < cg; c0 += wide) {
-    const int c = c0 + col;
+    float* __restrict__ sample, int S, int C, int cg, int gt, int nchunk) {
+  extern __shared__ float lds[];                // {u, u xhat} x channels, then {dz, dz xhat} x threads
+  const int G = C / cg;
+  const Join j(G, cg, gt);
+  const int at = j.g0 * cg;
+  const float* p = ws + j.b * nchunk * 2 * C + at;
+  float* share = lds + 2 * j.ch;
+  for (int c0 = 0; c0 < j.ch; c0 += 256) {
+    const int c = c0 + j.col;
     float a = 0.0f, d = 0.0f;
-    if (part < parts && c < cg)
-      for (int k = part; k < nchunk; k += parts) {
+    const bool on = j.part < j.parts && c < j.ch;
+    if (on) {
+      #pragma unroll 4
+      for (int k = j.part; k < nchunk; k += j.parts) {
         a += p[(int64_t)k * 2 * C + c];
         d += p[(int64_t)k * 2 * C + C + c];
       }
+    }
     __syncthreads();
-    lds[0][threadIdx.x] = a;
-    lds[1][threadIdx.x] = d;
+    share[threadIdx.x] = a;
+    share[256 + threadIdx.x] = d;
     __syncthreads();
-    if (part == 0 && c < cg) {
-      for (int k = 1; k < parts; ++k) {
-        a += lds[0][k * wide + col];
-        d += lds[1][k * wide + col];
+    if (on && j.part == 0) {
+      for (int k = 1; k < j.parts; ++k) {
+        a += share[k * j.ch + j.col];
+        d += share[256 + k * j.ch + j.col];
       }
-      sample[b * 2 * C + g * cg + c] = a;
-      sample[b * 2 * C + C + g * cg + c] = d;
-      const float wc = param<T>(w, f32, g * cg + c, 1.0f);
-      s1 += wc * a;
-      s2 += wc * d;
+      sample[j.b * 2 * C + at + c] = a;
+      sample[j.b * 2 * C + C + at + c] = d;
+      const float wc = param<T>(w, f32, at + c, 1.0f);
+      lds[c] = wc * a;
+      lds[j.ch + c] = wc * d;
     }
   }
-  s1 = faa_block_reduce_sum(s1, red);
   __syncthreads();
-  s2 = faa_block_reduce_sum(s2, red);
-  if (threadIdx.x == 0) {
-    const float count = (float)cg * (float)S;
-    means[2 * (int64_t)blockIdx.x] = s1 / count;
-    means[2 * (int64_t)blockIdx.x + 1] = s2 / count;
+  const int lane = threadIdx.x & 63;
+  const float count = (float)cg * (float)S;
+  for (int g = (int)threadIdx.x >> 6; g < j.groups; g += 4) {
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int c = lane; c < cg; c += 64) {
+      s1 += lds[g * cg + c];
+      s2 += lds[j.ch + g * cg + c];
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if (lane == 0) {
+      means[2 * (j.b * G + j.g0 + g)] = s1 / count;
+      means[2 * (j.b * G + j.g0 + g) + 1] = s2 / count;
+    }
   }
 }
 
@@ -823,6 +879,8 @@ Shape shape_of(const torch::Tensor& x, int64_t groups, const torch::Tensor& w, c
   const int64_t C = x.size(1), S = x.numel() ? x.numel() / (s.B * C) : 0;
   TORCH_CHECK(S * C < (int64_t(1) << 31), "group_norm_act: a sample has 2^31 values or more");
   TORCH_CHECK(C < (1 << 23), "group_norm_act: 2^23 channels or more");
+  // a channel's sums wait in LDS until its group is joined
+  TORCH_CHECK(groups <= 0 || C / groups <= 16384, "group_norm_act: a group has more than 16384 channels");
   TORCH_CHECK(groups > 0 && C > 0 && C % groups == 0, "group_norm_act: C is no multiple of the groups");
   s.S = (int)S;
   s.C = (int)C;
@@ -940,6 +998,9 @@ template <typename T, int VEC> constexpr int kBackwardR = VEC == 1 ? 32 : (VEC *
 
 constexpr int kR = 8;       // vectors a thread in a chunk
 
+// groups that one workgroup joins: lines of 32 channels, 128 bytes
+int join_groups(const Shape& s) { return std::min(s.G, std::max(1, 32 / s.cg)); }
+
 template <typename T, int VEC>
 void forward_on(const Shape& s, const torch::Tensor& x, const void* w, const void* b, bool f32,
              torch::Tensor& y, torch::Tensor& mean, torch::Tensor& rstd, double eps, int act,
@@ -961,9 +1022,11 @@ void forward_on(const Shape& s, const torch::Tensor& x, const void* w, const voi
   hipLaunchKernelGGL((gn_chunk_stats_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256), lds, stream,
                      (const T*)x.data_ptr(), ws.data_ptr<float>(), s.S, s.C, c.tile, c.ntile, c.nchunk,
                      c.chunk);
-  hipLaunchKernelGGL(gn_join_stats_kernel, dim3((unsigned)(s.B * s.G)), dim3(256), 0, stream,
-                     ws.data_ptr<float>(), mean.data_ptr<float>(), rstd.data_ptr<float>(), s.S, s.C,
-                     s.cg, c.nchunk, c.chunk, (float)eps);
+  const int gt = join_groups(s);
+  hipLaunchKernelGGL(gn_join_stats_kernel, dim3((unsigned)(s.B * ((s.G + gt - 1) / gt))), dim3(256),
+                     (2 * gt * s.cg + 768) * sizeof(float), stream, ws.data_ptr<float>(),
+                     mean.data_ptr<float>(), rstd.data_ptr<float>(), s.S, s.C, s.cg, gt, c.nchunk, c.chunk,
+                     (float)eps);
   hipLaunchKernelGGL((gn_chunk_apply_kernel<T, VEC, kR>), dim3((unsigned)c.wgs), dim3(256),
                      2 * c.tile * sizeof(float), stream, (const T*)x.data_ptr(), w, b, f32, mean.data_ptr<float>(), rstd.data_ptr<float>(),
                      (T*)y.data_ptr(), s.S, s.C, s.cg, c.tile, c.ntile, c.nchunk, c.chunk, act);
@@ -995,9 +1058,10 @@ torch::Tensor backward_on(const Shape& s, const torch::Tensor& dy, const torch::
                      (const T*)dy.data_ptr(), (const T*)x.data_ptr(), w, b, f32,
                      mean.data_ptr<float>(), rstd.data_ptr<float>(), ws.data_ptr<float>(), s.S, s.C,
                      s.cg, c.tile, c.ntile, c.nchunk, c.chunk, act);
-  hipLaunchKernelGGL((gn_join_grads_kernel<T>), dim3((unsigned)(s.B * s.G)), dim3(256), 0, stream,
-                     ws.data_ptr<float>(), w, f32, means.data_ptr<float>(), sample.data_ptr<float>(), s.S,
-                     s.C, s.cg, c.nchunk);
+  const int gt = join_groups(s);
+  hipLaunchKernelGGL((gn_join_grads_kernel<T>), dim3((unsigned)(s.B * ((s.G + gt - 1) / gt))), dim3(256),
+                     (2 * gt * s.cg + 512) * sizeof(float), stream, ws.data_ptr<float>(), w, f32,
+                     means.data_ptr<float>(), sample.data_ptr<float>(), s.S, s.C, s.cg, gt, c.nchunk);
   hipLaunchKernelGGL((gn_chunk_dx_kernel<T, VEC, kR, 4>), dim3((unsigned)c.wgs), dim3(256),
                      4 * c.tile * sizeof(float), stream,
                      (const T*)dy.data_ptr(), (const T*)x.data_ptr(), w, b, f32,

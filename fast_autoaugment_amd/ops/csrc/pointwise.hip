@@ -821,8 +821,9 @@ void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, t
                    && aligned(z->data_ptr(), 16)));
   const int vw = vec ? V : 1, tile = std::min(N, (vec ? 32 : 64) * vw), ntile = (N + tile - 1) / tile;
   const int rows = 256 / (tile / vw);
-  // about 2048 workgroups, and chunks of 16 rows a thread at least
-  int64_t chunk = std::max<int64_t>(16, (M * ntile / 2048 + rows - 1) / rows) * rows;
+  // 1024 workgroups or more, as long as a thread has 4 rows; few rows are one chunk, whose sums need no joining
+  int64_t chunk = std::max<int64_t>(4, M * ntile / 1024 / rows) * rows;
+  if (M <= 16 * rows) chunk = 16 * rows;
   chunk = std::min<int64_t>(chunk, 1 << 24);
   const int64_t chunks = (M + chunk - 1) / chunk;
   TORCH_CHECK(chunks * ntile < (int64_t(1) << 24), "linear_act: too many rows");
