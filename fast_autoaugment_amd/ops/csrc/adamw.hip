@@ -147,8 +147,8 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// part[block] = sum of squares of the block's chunks, added in a fixed order. 16 values are added in fp32, all
-// else in 64 bits: an error of the norm would move every gradient the same way, and 8-bit moments over a border.
+// part[block] = sum of squares of the block's chunks, added in a fixed order and in 64 bits: an error of the norm
+// would move every gradient the same way, and 8-bit moments over a border.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(
     const int64_t* __restrict__ rows, const int* __restrict__ chunks, int n_chunks,
@@ -159,13 +159,12 @@ __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(
     Row r = read_row(rows, chunks[2 * c]);
     if (r.g == nullptr) continue;
     int64_t base = (int64_t)chunks[2 * c + 1] * kChunk + threadIdx.x * 4;
-    float s = 0.0f;
     #pragma unroll
     for (int it = 0; it < kIters; ++it) {
       f32x4 g = load4((const T*)r.g, base + it * kThreads * 4, r.n, r.aligned);
-      s += (g[0] * g[0] + g[1] * g[1]) + (g[2] * g[2] + g[3] * g[3]);
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) acc += (double)(g[i] * g[i]);
     }
-    acc += (double)s;
   }
   acc = wave_sum(acc);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = acc;
@@ -190,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void adamw_begin_kernel(
   if (threadIdx.x == 0) {
     step[0] += 1;
     float norm = (float)sqrt(lds[0] + lds[1] + lds[2] + lds[3]);
-    scal[0] = clip > 0.0f ? fminf(1.0f, clip / (norm + 1e-6f)) : 1.0f;
+    scal[0] = clip > 0.0f ? fminf(1.0f, clip * (1.0f / (norm + 1e-6f))) : 1.0f;
     if (norm != norm) scal[0] = norm;     // fminf would hide a norm that is no number
   }
 }
@@ -209,6 +208,9 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(
     const int64_t* __restrict__ rows, const int* __restrict__ chunks, Moments st,
     const float* __restrict__ scal, const float* __restrict__ lr_p,
     float b1, float c1, float b2, float c2, float eps) {
+  // Every operation is rounded by itself and in the CPU path's order, so that moments held in 8 bits are that
+  // path's bit for bit: a fused product and sum would leave some of them on the other side of a border.
+  #pragma clang fp contract(off)
   const Row r = read_row(rows, chunks[2 * blockIdx.x]);
   if (r.g == nullptr) return;             // no gradient: the tensor is left as it is
   const int64_t base = (int64_t)chunks[2 * blockIdx.x + 1] * kChunk + threadIdx.x * 4;
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(
     for (int i = 0; i < 4; ++i) {
       const float gg = g[it][i] * coef;
       mm[i] = b1 * mm[i] + c1 * gg;
-      vv[i] = b2 * vv[i] + c2 * gg * gg;
+      vv[i] = b2 * vv[i] + (c2 * gg) * gg;
       root[i] = sqrtf(vv[i]);
       pp[i] = pp[i] * keep - lr * (mm[i] * a1 / (root[i] * a2 + eps));
     }
@@ -267,16 +269,16 @@ __global__ __launch_bounds__(kThreads) void adamw_step_kernel(
       tm = fmaxf(wave_max(tm), kQTiny);
       tr = fmaxf(wave_max(tr), kQTiny);
       if (e < r.n) {
-        uint32_t um = to_e4m3(mm * (kQMax / tm));
-        uint32_t ur = to_e4m3(root * (kQMax / tr));
+        uint32_t um = to_e4m3(mm * (kQMax * (1.0f / tm)));
+        uint32_t ur = to_e4m3(root * (kQMax * (1.0f / tr)));
         #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (root[i] > 0.0f && ((ur >> (8 * i)) & 0xff) == 0) ur |= 1u << (8 * i);
         *(uint32_t*)((uint8_t*)st.m + r.off + e) = um;
         *(uint32_t*)((uint8_t*)st.r + r.off + e) = ur;
         if ((threadIdx.x & 63) == 0) {
-          st.ms[(r.off + e) / kBlock] = tm / kQMax;
-          st.rs[(r.off + e) / kBlock] = tr / kQMax;
+          st.ms[(r.off + e) / kBlock] = tm * (1.0f / kQMax);
+          st.rs[(r.off + e) / kBlock] = tr * (1.0f / kQMax);
         }
       }
     }

@@ -487,7 +487,7 @@ class FusedAdamW:
                          self._part, self._lr_t, self.betas[0], self.betas[1], self.eps,
                          self.grad_clip)
 
-    # ---- CPU reference path (defines the kernels' semantics)
+    # ---- CPU reference path (defines the kernels' semantics: they round each of these operations alike)
 
     def _moment(self, name, off, n):
         if self.state_bits == 32:
@@ -506,21 +506,22 @@ class FusedAdamW:
         v = v.view(-1, self.BLOCK)
         finite = torch.nan_to_num(v.abs(), nan=0.0, posinf=math.inf)
         top = finite.amax(1, keepdim=True).clamp_min(2.0 ** -100)
-        q = (v * (448.0 / top)).to(torch.float8_e4m3fn)
+        q = (v * (top.reciprocal() * 448.0)).to(torch.float8_e4m3fn)
         if least:
             q = torch.where((v > 0) & (q.float() == 0), torch.tensor(2.0 ** -9), q.float()).to(torch.float8_e4m3fn)
         getattr(self, name).view(torch.uint8)[lo * self.BLOCK:hi * self.BLOCK] = q.view(-1).view(torch.uint8)
-        getattr(self, name + "_scale")[lo:hi] = (top / 448.0).view(-1)
+        getattr(self, name + "_scale")[lo:hi] = (top * (1.0 / 448.0)).view(-1)
 
     def _step_cpu(self):
         (b1, b2), lr = self.betas, self.lr
         views = self._views()
         self.step_count += 1
         t = int(self.step_count)
-        coef = 1.0
+        coef = torch.ones(())
         if self.grad_clip > 0:
-            sq = sum(float(g.double().square().sum()) for _, _, _, g, *_ in views if g is not None)
-            coef = min(1.0, self.grad_clip / (math.sqrt(sq) + 1e-6)) if sq == sq else math.nan
+            sq = sum(float(g.float().square().sum(dtype=torch.float64)) for _, _, _, g, *_ in views if g is not None)
+            norm = torch.tensor(math.sqrt(sq) if sq == sq else math.nan)
+            coef = ((norm + 1e-6).reciprocal() * self.grad_clip).clamp_max(1.0)
         second = "exp_avg_sq" if self.state_bits == 32 else "exp_avg_root"
         flat = lambda x: x.as_strided((x.numel(),), (1,))  # noqa: E731
         for _, w, low, g, off, n, wd in views:
@@ -529,8 +530,8 @@ class FusedAdamW:
             gf = flat(g).float() * coef
             m = b1 * self._moment("exp_avg", off, n) + (1 - b1) * gf
             v = self._moment(second, off, n)
-            v = b2 * (v if self.state_bits == 32 else v.square()) + (1 - b2) * gf * gf
-            root = v.sqrt()
+            v = b2 * (v if self.state_bits == 32 else v.square()) + ((1 - b2) * gf) * gf
+            root = v.double().sqrt().float()       # torch's fp32 root on the CPU is off by a step at times
             wf = flat(w)
             wf.mul_(1 - lr * wd).sub_(lr * (m / (1 - b1 ** t)) / (root / math.sqrt(1 - b2 ** t) + self.eps))
             if low is not None:

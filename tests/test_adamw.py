@@ -301,6 +301,23 @@ def test_captured_steps_follow_eager_ones(bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [0.0, 0.5])
+def test_the_gpu_s_moments_are_the_cpu_s(bits, clip):
+    """Bit for bit, over steps that build on each other: a rounding more or less would show in 8 bits now and then."""
+    out = []
+    for dev in ("cpu", "cuda"):
+        p = nn.Parameter(tensors(torch.bfloat16, dev, shapes=[(200_000,)])[0])
+        opt = FusedAdamW([p], lr=1e-2, weight_decay=0.1, grad_clip=clip, state_bits=bits)
+        for step in range(4):
+            p.grad = tensors(torch.bfloat16, dev, seed=30 + step, shapes=[(200_000,)])[0]
+            opt.step()
+        out.append([getattr(opt, k).float().cpu() for k in opt._names])
+    for x, y in zip(*out):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
 def test_gpu_refusals():
     p = nn.Parameter(torch.zeros(300, device="cuda"))
     p.grad = torch.ones(300, device="cuda")
