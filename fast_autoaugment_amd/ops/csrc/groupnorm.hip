@@ -918,7 +918,7 @@ Chunks chunks_of(const Shape& s, int R) {
   c.ntile = (s.C + c.tile - 1) / c.tile;
   const int rows = 256 / (c.tile / VEC);
   c.chunk = rows * R;
-  c.nchunk = (s.S + c.chunk - 1) / c.chunk;
+  c.nchunk = (int)(((int64_t)s.S + c.chunk - 1) / c.chunk);
   c.wgs = s.B * c.ntile * c.nchunk;
   TORCH_CHECK(c.wgs < (int64_t(1) << 24) && s.B * s.G < (int64_t(1) << 24),
               "group_norm_act: more workgroups than a launch takes");     // 2^32 threads
@@ -947,11 +947,12 @@ template <typename T, int VEC, int MOST_R>
 bool whole_of(const Shape& s, Whole& out) {
   const int64_t unit = std::lcm((int64_t)s.cg, (int64_t)VEC), line = sizeof(T) * unit;
   if ((int64_t)s.S * s.C * sizeof(T) >= (int64_t(1) << 30) || unit / VEC > 256) return false;   // offsets: 32 bits
-  const int64_t units = s.C / unit, sixteen = 16 / sizeof(T);
+  // at most 2048 channels a workgroup: their constants share LDS with the threads' sums (131 KB backward)
+  const int64_t units = s.C / unit, sixteen = 16 / sizeof(T), most = std::max<int64_t>(1, 2048 / unit);
   auto vectors = [&](int64_t k) { return k * unit * s.S / sixteen; };
   auto workgroups = [&](int64_t k) { return s.B * ((units + k - 1) / k); };
   auto lines = [&](int64_t bytes) { return std::min(units, std::max<int64_t>(1, bytes / line)); };
-  int64_t k = std::min(units, std::max(lines(64), 2048 / std::max<int64_t>(1, vectors(1))));
+  int64_t k = std::min({units, most, std::max(lines(64), 2048 / std::max<int64_t>(1, vectors(1)))});
   for (int bytes : {128, 64, 32})
     while (k > lines(bytes) && workgroups(k) < 8 * bytes) k = std::max(lines(bytes), k / 2);
   if (vectors(k) > 4096) {

@@ -120,6 +120,15 @@ def test_fp32_parameters_with_low_precision_maps(dev):
     check(dev, x, 4, w, b, "swish", dy)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((1100, 8192), 1024), ((1100, 8192, 1, 1), 8192), ((1030, 6144, 1, 2), 768),
+                                          ((1030, 2600, 1, 1), 650)])
+def test_many_channels_and_few_pixels(shape, groups):
+    """Whole samples fit a workgroup's registers here, but the constants of their channels are more than LDS."""
+    x, w, b, dy = inputs(shape, BF16)
+    check("cuda", x, groups, w, b, "relu", dy)
+
+
 @pytest.mark.parametrize("dev", DEV)
 @pytest.mark.parametrize("shape,groups", [((2, 16, 40, 40), 2), ((2, 16, 150, 150), 2), ((2, 15, 20, 20), 3)])
 def test_a_mean_far_from_zero(dev, shape, groups):
