@@ -108,14 +108,15 @@ __device__ __forceinline__ float act_value(float z) {
   if (ACT == ACT_SWISH) return z * sigmoid(z);
   return z;
 }
+// d times the slope at z; where relu holds back, no infinity or NaN of d comes through
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+__device__ __forceinline__ float act_grad(float d, float z) {
+  if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : d;
   if (ACT == ACT_SWISH) {
     const float s = sigmoid(z);
-    return s + s * (z - z * s);
+    return d * (s + s * (z - z * s));
   }
-  return 1.0f;
+  return d;
 }
 // f(activation as a constant): one branch outside the loops, not one an element
 template <typename F>
@@ -521,7 +522,7 @@ __global__ __launch_bounds__(256) void gn_chunk_grads_kernel(
             #pragma unroll
             for (int j = 0; j < VEC; ++j) {
               const float xv = P::get(xr[i], j);
-              const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+              const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
               acc[0][j] += dz;
               acc[1][j] += dz * xv;
             }
@@ -644,7 +645,7 @@ __global__ __launch_bounds__(256) void gn_chunk_dx_kernel(
           #pragma unroll
           for (int j = 0; j < VEC; ++j) {
             const float xv = P::get(xr[i], j);
-            const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+            const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
             P::set(out, j, dz * a[j] + (xv * pp[j] + q[j]));
           }
           store_at<T, VEC>(dx + at, off + (o + i) * step, out);
@@ -778,7 +779,7 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
         #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float xv = P::get(xr[i], j);
-          const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+          const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
           acc[0][j] += dz;
           acc[1][j] += dz * xv;
         }
@@ -816,7 +817,7 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
         #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float xv = P::get(xr[i], j);
-          const float dz = P::get(dr[i], j) * act_slope<A.value>(xv * a[j] + c[j]);
+          const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
           P::set(out, j, dz * a[j] + (xv * pp[j] + q[j]));
         }
         store_at<T, VEC>(dx + at, off + i * step, out);

@@ -123,14 +123,15 @@ __device__ __forceinline__ float act_value(float z) {
   if (ACT == ACT_SIGMOID) return sigmoid(z);
   return z;
 }
-// from z, or for relu from y: both are above 0 in the same places, but for z below half the type's smallest number
+// d times the slope at z, or for relu at y: both are above 0 in the same places, but for z below half the type's
+// smallest number. Where relu holds back, no infinity or NaN of d comes through.
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if (ACT == ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+__device__ __forceinline__ float act_grad(float d, float z) {
+  if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : d;
   const float s = sigmoid(z);
-  if (ACT == ACT_SWISH) return s + s * (z - z * s);
-  if (ACT == ACT_SIGMOID) return s - s * s;
-  return 1.0f;
+  if (ACT == ACT_SWISH) return d * (s + s * (z - z * s));
+  if (ACT == ACT_SIGMOID) return d * (s - s * s);
+  return d;
 }
 // f(activation as a constant): one branch outside the loops, not one an element
 template <bool ANY = true, typename F>
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
           #pragma unroll
           for (int h = 0; h < H; ++h) {
             #pragma unroll
-            for (int i = 0; i < E; ++i) d[h][i] *= act_slope<A.value>(zz[h][i]);
+            for (int i = 0; i < E; ++i) d[h][i] = act_grad<A.value>(d[h][i], zz[h][i]);
             store4(dz + at + 4 * h, E, VEC > 1, d[h]);
           }
         }

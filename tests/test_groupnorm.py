@@ -159,6 +159,21 @@ def test_what_is_no_number_stays_in_its_group(dev):
 
 
 @pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("shape", [(2, 16, 8, 8), (2, 16, 130, 130)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_relu_holds_back_gradients_that_are_no_numbers(dev, shape, bad):
+    x, w, b, dy = inputs(shape, FP32)
+    grads = []
+    for fill in (0.0, bad):
+        leaves = [t.to(dev).requires_grad_(True) for t in (x, w, b)]
+        y = group_norm_act(leaves[0], 4, leaves[1], leaves[2], act="relu")
+        assert (y == 0).any()
+        grads.append(torch.autograd.grad(y, leaves, torch.where(y.detach() == 0, fill, dy.to(dev))))
+    for a, c in zip(*grads):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dev", DEV)
 def test_orders_of_memory(dev):
     x, w, b, dy = inputs((2, 16, 6, 7), BF16)
     for layout in (lambda v: v, lambda v: v.contiguous(memory_format=torch.channels_last),

@@ -162,6 +162,23 @@ def test_what_is_no_number_stays_in_its_row(dev):
 
 
 @pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("t", [FP32, BF16])
+@pytest.mark.parametrize("n", [40, 33])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_relu_holds_back_gradients_that_are_no_numbers(dev, t, n, bad):
+    g = torch.Generator().manual_seed(5)
+    x, w, b, r, dy = (torch.randn(*s, generator=g).to(t).to(dev) for s in ((70, 24), (n, 24), (n,), (70, n), (70, n)))
+    grads = []
+    for fill in (0.0, bad):
+        leaves = [v.clone().requires_grad_(True) for v in (x, w, b, r)]
+        y = linear_act(*leaves, act="relu")
+        assert (y == 0).any()
+        grads.append(torch.autograd.grad(y, leaves, torch.where(y.detach() == 0, torch.tensor(fill, dtype=t, device=dev), dy)))
+    for a, c in zip(*grads):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dev", DEV)
 def test_only_what_is_asked_for(dev):
     x, w, b, r, dy = (t.to(dev) for t in inputs(200, 72, 40, BF16))
     full = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
