@@ -72,18 +72,22 @@ torch::Tensor dwconv_bwd_data(torch::Tensor dy, torch::Tensor w, int64_t stride,
 torch::Tensor dwconv_bwd_weight(torch::Tensor dy, torch::Tensor x, int64_t stride,
                                 int64_t pt, int64_t pl, int64_t KH, int64_t KW);
 
-// what device tables of addresses depend on: place, size and memory order of every tensor and of its gradient
+// what device tables of addresses depend on: place, type, size and memory order of every tensor and of its gradient
 static py::bytes tensor_addresses(const std::vector<torch::Tensor>& ts) {
   std::vector<int64_t> a;
   a.reserve(ts.size() * 16);
   for (const auto& t : ts) {
     a.push_back((int64_t)t.data_ptr());
+    a.push_back((int64_t)t.scalar_type());
     a.insert(a.end(), t.sizes().begin(), t.sizes().end());
     a.insert(a.end(), t.strides().begin(), t.strides().end());
     const auto& g = t.grad();
     const bool strided = g.defined() && g.layout() == torch::kStrided;
     a.push_back(strided ? (int64_t)g.data_ptr() : g.defined() ? -1 : 0);
-    if (strided) a.insert(a.end(), g.strides().begin(), g.strides().end());
+    if (strided) {
+      a.push_back((int64_t)g.scalar_type());
+      a.insert(a.end(), g.strides().begin(), g.strides().end());
+    }
   }
   return py::bytes((const char*)a.data(), a.size() * sizeof(int64_t));
 }

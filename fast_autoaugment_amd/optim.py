@@ -395,8 +395,9 @@ class FusedAdamW:
             if n == 0:
                 continue
             w, low = (p.detach(), None) if master is None else (master, p.detach())
-            if p.numel() != n or p.device != self._dev or not self._same_order(p, w):
-                raise ValueError("FusedAdamW: a parameter is not contiguous, or changed its size, device or order")
+            if (p.numel() != n or p.device != self._dev or (p.dtype == torch.float32) != (low is None)
+                    or not self._same_order(p, w)):
+                raise ValueError("FusedAdamW: a parameter is not contiguous, or changed its size, type, device or order")
             g = p.grad
             if g is not None:
                 if g.layout != torch.strided or g.dtype != p.dtype or g.device != self._dev or g.shape != p.shape:

@@ -335,6 +335,21 @@ def test_gpu_refusals():
         FusedAdamW([nn.Parameter(torch.zeros(3, device="cuda")), nn.Parameter(torch.zeros(3))])
 
 
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("before,after", [(torch.float32, torch.bfloat16), (torch.float16, torch.float32)])
+def test_a_parameter_that_changes_its_type_is_refused(dev, before, after):
+    """Its fp32 weights would be read from memory of another type and length."""
+    p = nn.Parameter(tensors(before, dev, shapes=[(5000,)])[0])
+    opt = FusedAdamW([p])
+    p.grad = torch.zeros_like(p)
+    opt.step()
+    p.grad = None
+    p.data = p.data.to(after)
+    p.grad = torch.zeros_like(p)
+    with pytest.raises((TypeError, ValueError), match="changed its size, type"):
+        opt.step()
+
+
 @pytest.mark.gpu
 def test_a_captured_step_outlives_new_gradients():
     """A graph keeps the tables it was captured with, whatever eager steps on other gradients make later."""
