@@ -72,13 +72,15 @@ torch::Tensor dwconv_bwd_data(torch::Tensor dy, torch::Tensor w, int64_t stride,
 torch::Tensor dwconv_bwd_weight(torch::Tensor dy, torch::Tensor x, int64_t stride,
                                 int64_t pt, int64_t pl, int64_t KH, int64_t KW);
 
-// what device tables of addresses depend on: place, type, size and memory order of every tensor and of its gradient
+// what device tables of addresses depend on: place, type, size and memory order of every tensor and of its gradient,
+// and whether a low-precision tensor was written
 static py::bytes tensor_addresses(const std::vector<torch::Tensor>& ts) {
   std::vector<int64_t> a;
   a.reserve(ts.size() * 16);
   for (const auto& t : ts) {
     a.push_back((int64_t)t.data_ptr());
     a.push_back((int64_t)t.scalar_type());
+    a.push_back(t.scalar_type() == torch::kFloat32 || t.is_inference() ? 0 : (int64_t)t._version());
     a.insert(a.end(), t.sizes().begin(), t.sizes().end());
     a.insert(a.end(), t.strides().begin(), t.strides().end());
     const auto& g = t.grad();

@@ -267,8 +267,10 @@ class FusedAdamW:
     ``{"params": [...], "weight_decay": w}`` groups. Parameters are contiguous,
     fp32, bf16 or fp16, and all on one device; bf16 and fp16 ones get fp32
     weights that the optimizer keeps (FlatParams brings its own), which are
-    updated and rounded back into the parameters. A parameter whose ``grad`` is
-    None is left as it is. The step count is one for all parameters.
+    updated and rounded back into the parameters. Such a parameter that was
+    written since the last step (a checkpoint that was loaded) is taken over
+    where it is not its fp32 weight rounded; a write through ``p.data`` is not
+    seen. A parameter whose ``grad`` is None is left as it is. The step count is one for all parameters.
 
     ``state_bits=8`` holds m and sqrt(v) as e4m3 numbers (``exp_avg``,
     ``exp_avg_root``) with one fp32 scale for every 256 neighbours of a tensor
@@ -374,7 +376,13 @@ class FusedAdamW:
         if any(p.device != self._dev for p in self.params):
             raise ValueError("FusedAdamW: the parameters are on several devices")
         self.masters = [None if p.dtype == torch.float32 else p.detach().float() for p in self.params]
+        self._stamps = [self._stamp(p) for p in self.params]
         return total
+
+    @staticmethod
+    def _stamp(p):
+        """What changes when a tensor is written by torch or put elsewhere."""
+        return p.data_ptr(), 0 if p.is_inference() else p._version
 
     @staticmethod
     def _same_order(a, b):
@@ -391,13 +399,16 @@ class FusedAdamW:
             return [(f.flat_param.dtype, full[off:off + n], None if low is None else low[off:off + n],
                      f.flat_grad[off:off + n], off, n, wd) for off, n, wd in self._items if n > 0]
         views = []
-        for p, master, (off, n, wd) in zip(self.params, self.masters, self._items):
+        for i, (p, master, (off, n, wd)) in enumerate(zip(self.params, self.masters, self._items)):
             if n == 0:
                 continue
             w, low = (p.detach(), None) if master is None else (master, p.detach())
             if (p.numel() != n or p.device != self._dev or (p.dtype == torch.float32) != (low is None)
                     or not self._same_order(p, w)):
                 raise ValueError("FusedAdamW: a parameter is not contiguous, or changed its size, type, device or order")
+            if low is not None and self._stamp(p) != self._stamps[i]:
+                w.copy_(torch.where(w.to(low.dtype) == low, w, low.float()))
+                self._stamps[i] = self._stamp(p)
             g = p.grad
             if g is not None:
                 if g.layout != torch.strided or g.dtype != p.dtype or g.device != self._dev or g.shape != p.shape:
@@ -424,8 +435,8 @@ class FusedAdamW:
                 self._captured.append(self._tables)     # a graph reads them as long as it is replayed
             return self._tables
         if capturing:
-            raise RuntimeError("FusedAdamW: the gradients' addresses changed since the last eager step: "
-                               "keep them in place (zero_grad() fills them) and step once before capture")
+            raise RuntimeError("FusedAdamW: the gradients' addresses changed since the last eager step, or parameters "
+                               "were written: keep gradients in place (zero_grad() fills them) and step once before capture")
         by = {}
         for kind, w, low, g, off, n, wd in self._views():
             rows, lengths = by.setdefault(self._KINDS[kind], ([], []))
@@ -539,6 +550,8 @@ class FusedAdamW:
                 flat(low).copy_(wf)
             self._hold("exp_avg", off, n, m, False)
             self._hold(second, off, n, v if self.state_bits == 32 else root, True)
+        if self.flat is None:
+            self._stamps = [self._stamp(p) for p in self.params]
 
     def state_dict(self):
         sd = {"step": int(self.step_count), "lr": self.lr, "state_bits": self.state_bits}

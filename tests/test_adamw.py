@@ -350,6 +350,27 @@ def test_a_parameter_that_changes_its_type_is_refused(dev, before, after):
         opt.step()
 
 
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_weights_that_were_loaded_are_taken_over(dev, bits):
+    """Weights loaded behind the optimizer's back are stepped from, and those it wrote itself keep their fp32 digits."""
+    p = nn.Parameter(tensors(torch.bfloat16, dev, shapes=[(5000,)])[0])
+    opt = FusedAdamW([p], lr=1e-3, state_bits=bits)
+    for step in range(3):
+        p.grad = torch.ones_like(p)
+        opt.step()
+        held = opt.masters[0].clone()
+        with torch.no_grad():
+            p[:2000] = 3.0
+        opt.lr = opt.param_groups[0]["lr"] = 0.0
+        opt.step()
+        # a step of lr 1e-3 from 3 still rounds to 3 in bf16 (its numbers lie 2^-6 apart there), and is kept
+        want = torch.where(held[:2000].bfloat16() == 3.0, held[:2000], 3.0)
+        assert torch.equal(opt.masters[0], torch.cat([want, held[2000:]])) and (p.detach()[:2000] == 3.0).all()
+        opt.param_groups[0]["lr"] = 1e-3
+    assert not torch.equal(held[2000:], held[2000:].bfloat16().float())
+
+
 @pytest.mark.gpu
 def test_a_captured_step_outlives_new_gradients():
     """A graph keeps the tables it was captured with, whatever eager steps on other gradients make later."""
