@@ -32,7 +32,8 @@ def _cached_model(conf, nc, save_path: str, device: str):
     import os as _os
     # fold_inference: the frozen child's 1x1 convolutions with their BatchNorm, skip and activation as one product
     fold = bool(conf.get_value("fold_inference", False))
-    key = (save_path, conf["model"].get("type"), nc, fold)
+    key = (save_path, tuple(conf["model"].get(k) for k in ("type", "norm", "norm_groups")), nc, fold,
+           conf.get_value("precision", "bf16"))
     mtime = _os.path.getmtime(save_path)
     hit = _MODEL_CACHE.get(key)
     if hit is not None and hit[0] == mtime:

@@ -245,3 +245,17 @@ def test_the_search_scores_a_folded_child(tmp_path):
         os.environ.pop("FAA_SYNTH_TEST", None)
         data_api._STORE_CACHE.clear()
         density_match._MODEL_CACHE.clear()
+
+
+def test_a_child_of_another_norm_is_not_the_cached_one(tmp_path):
+    """Group norms of other group counts load the same checkpoint, but are other networks."""
+    from fast_autoaugment_amd.search.density_match import _cached_model
+    path = str(tmp_path / "child.pth")
+    torch.save(build_model({"type": "wresnet40_2", "norm": "group"}, 10).state_dict(), path)
+    groups = set()
+    for n in (8, 4):
+        conf = C()
+        conf["model"] = {"type": "wresnet40_2", "norm": "group", "norm_groups": n}
+        model = _cached_model(conf, 10, path, "cpu")
+        groups.add(max(m.num_groups for m in model.modules() if isinstance(m, torch.nn.GroupNorm)))
+    assert groups == {8, 4}
