@@ -24,6 +24,7 @@
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <hip/hip_fp16.h>
@@ -333,6 +334,8 @@ void adamw_step(std::vector<torch::Tensor> rows, std::vector<torch::Tensor> chun
                 && chunks[i].size(1) == 2 && chunks[i].device() == m.device()
                 && chunks[i].is_contiguous(), "adamw_step: chunks");
     TORCH_CHECK(kinds[i] >= 0 && kinds[i] <= 2, "adamw_step: kind");
+    // the caller may let go of the tables while this stream, which need not be theirs, still reads them
+    for (const auto& t : {rows[i], chunks[i]}) t.record_stream(at::hip::getCurrentHIPStreamMasqueradingAsCUDA());
     if (clip <= 0.0 || chunks[i].size(0) == 0) continue;
     const int nc = (int)chunks[i].size(0), grid = std::min(nc, per);
     TORCH_CHECK(grid > 0, "adamw_step: part is too short");

@@ -457,9 +457,6 @@ class FusedAdamW:
         up = lambda t: t.contiguous().pin_memory().to(self._dev, non_blocking=True)  # noqa: E731
         rows = [up(torch.tensor(r, dtype=torch.int64).view(-1, 6)) for r, _ in by.values()]
         chunks = [up(chunk_table(n)) for _, n in by.values()]
-        if self._tables is not None:    # the old ones may still be read on this stream
-            for t in self._tables[0] + self._tables[1]:
-                t.record_stream(torch.cuda.current_stream(self._dev))
         self._tables = (rows, chunks, list(by))
         self._seen = self._addresses()
         return self._tables
