@@ -21,6 +21,11 @@
 //
 // The step count, learning rate and clip factor live on the device, so a step
 // can be captured and replayed.
+//
+// Bound by memory. 36.5M bf16 parameters with fp32 weights: with 32-bit moments
+// 28 bytes an element in 187 us, 5.5 TB/s; with 8-bit moments 16 bytes in 116 us,
+// 5.0 TB/s (a copy reaches 4.9). A clip factor needs all gradients first: 73 MB
+// in 26 us. 36 tensors of 16 to 147456 elements take 8 us, and 3 for the scalars.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>

@@ -20,6 +20,14 @@
 //
 // Operands whose lines do not start at 16 bytes are first copied into lines
 // that do, which costs less than loads of 2 bytes in the product.
+//
+// The models' products are bound by memory: 100352x128x512 with residual and
+// relu takes 60 us for 231 MB, 3.9 TB/s (a copy reaches 4.9; with two steps of k
+// a workgroup's load, product and store hardly overlap). 25088x1024x256 trained
+// takes 24 + 28 + 27 us (y, dx, dW) and 15 for dz and its sums. Results that are
+// turned in LDS, to leave as lines of 128 bytes, took 98.7 us for 104.6
+// (401408x64x256 with residual), but 40.6 for 35.1 (100352x128x512 without).
+// Products of a few hundred rows take 3 to 6 us, which is a launch.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -763,9 +771,15 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
   int BM = 64, BN = 64, step = 16;
   if constexpr (sizeof(T) == 2) {
     step = BK;
+    // Large tiles read less, small ones fill the card: 128 x 128 or 128 x 64 where there are 384 of them, or where so
+    // few (128 x 128) that k is split and a part still has 16 steps. Measured (us, 128x128/128x64/64x64, M x N, K):
+    // 25088x256, 1024 (392 tiles of 128x128) 21/24/24; 100352x512, 128 33/35/38; 6272x512, 2048 (196) 24/22/25;
+    // 16384x130, 200 (256) 11.0/10.5/9.4; 2048x1000, 1280 (128) 24/12/11; and split, 256x1024, 25088 27/27/35;
+    // 2048x512, 6272 27/27/32; 512x128, 100352 46/51/62; but 256x256, 8192 (2 steps) 16/15/11; 256x64, 401408 77/76/69.
     auto tiles = [&](int64_t a, int64_t b) { return ((M + a - 1) / a) * ((N + b - 1) / b); };
-    if (M > 64 && (tiles(128, 64) >= 256 || K >= 8192)) BM = 128;
-    if (BM == 128 && N > 64 && (tiles(128, 128) >= 256 || K >= 8192)) BN = 128;
+    const int64_t large = tiles(128, 128);
+    if (M > 64 && N > 64 && (large >= 384 || (large <= 128 && (K + BK - 1) / BK * large >= 16 * 256))) BM = BN = 128;
+    else if (M > 64 && tiles(128, 64) >= 384) BM = 128;
   }
   const int64_t tm = (M + BM - 1) / BM, tn = (N + BN - 1) / BN, steps = (K + step - 1) / step;
   // few tiles and a long k: parts for one workgroup a CU, each with 4 steps at least. More parts are more fp32 to
@@ -822,7 +836,8 @@ void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, t
                    && aligned(z->data_ptr(), 16)));
   const int vw = vec ? V : 1, tile = std::min(N, (vec ? 32 : 64) * vw), ntile = (N + tile - 1) / tile;
   const int rows = 256 / (tile / vw);
-  // 1024 workgroups or more, as long as a thread has 4 rows; few rows are one chunk, whose sums need no joining
+  // 1024 workgroups or more, as long as a thread has 4 rows (25088x256 takes 10 us, with fewer 16); few rows are
+  // one chunk, whose sums need no joining
   int64_t chunk = std::max<int64_t>(4, M * ntile / 1024 / rows) * rows;
   if (M <= 16 * rows) chunk = 16 * rows;
   chunk = std::min<int64_t>(chunk, 1 << 24);
