@@ -27,6 +27,9 @@
 // takes 24 + 28 + 27 us (y, dx, dW) and 15 for dz and its sums. Results that are
 // turned in LDS, to leave as lines of 128 bytes, took 98.7 us for 104.6
 // (401408x64x256 with residual), but 40.6 for 35.1 (100352x128x512 without).
+// Stores past the caches are faster for a product alone (59 us for 63 a call), but
+// what reads the result next pays for them: 25088x1024x256 and a product back
+// 53 for 47.
 // Products of a few hundred rows take 3 to 6 us, which is a launch.
 
 #include <torch/extension.h>

@@ -427,3 +427,30 @@ def test_odd_lengths(dev, n, bits):
         before = state_of(opt, [p])
         opt.step()
         check_step(opt, before, [p.grad], [p], [0.1], 1e-2, 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_beyond_32_bits(bits):
+    """The end of a tensor of more than 2^31 elements, and the tensor behind it, are stepped as they are alone."""
+    g = torch.Generator("cuda").manual_seed(3)
+    r = lambda n: torch.randn(n, generator=g, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    n = 2 ** 31 + 3 * 4096
+    weights, grads = [r(n), r(5000)], [r(n), r(5000)]
+    end = slice(n - 8192, None)
+    got = []
+    for ws, gs in ((weights, grads), ([weights[0][end].clone(), weights[1].clone()], [grads[0][end].clone(), grads[1]])):
+        ps = [nn.Parameter(w.clone()) for w in ws]
+        for p, grad in zip(ps, gs):
+            p.grad = grad
+        opt = FusedAdamW(ps, lr=1e-2, weight_decay=0.1, state_bits=bits)
+        opt.step()
+        opt.step()
+        held = [getattr(opt, k) for k in opt._names]
+        held = [h[-(8192 + 5120) // 256:].float() if k.endswith("scale") else h[-(8192 + 5120):].float()
+                for k, h in zip(opt._names, held)]
+        got.append([ps[0].detach()[-8192:], ps[1].detach(), opt.masters[0][-8192:], *held])
+        del ps, opt
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+

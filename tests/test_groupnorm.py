@@ -294,3 +294,23 @@ def test_two_streams_at_once():
     for i in range(2):
         for y in got[i]:
             assert torch.equal(y, alone[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((2200, 1024, 31, 31), 32), ((12, 256, 840, 840), 4)])
+def test_offsets_beyond_32_bits(shape, groups):
+    """The last samples of a map of more than 2^31 values are what they are by themselves."""
+    g = torch.Generator("cuda").manual_seed(3)
+    make = lambda: torch.randn(shape[0], *shape[2:], shape[1], generator=g, device="cuda",  # noqa: E731
+                               dtype=BF16).movedim(-1, 1)
+    x, dy = make().requires_grad_(True), make()
+    assert x.numel() * 2 > 2 ** 32
+    w = torch.rand(shape[1], generator=g, device="cuda", dtype=torch.float32).to(BF16) + 0.5
+    y = group_norm_act(x, groups, w, act="swish")
+    dx, = torch.autograd.grad(y, x, dy)
+    last = x.detach()[-2:].clone(memory_format=torch.channels_last).requires_grad_(True)
+    y2 = group_norm_act(last, groups, w, act="swish")
+    dx2, = torch.autograd.grad(y2, last, dy[-2:])
+    # one sample's sums may be cut in other parts there: a step of bf16, and of values near 0 one of those near 1
+    for a, b in ((y[-2:], y2), (dx[-2:], dx2)):
+        assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -12)

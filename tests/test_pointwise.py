@@ -257,3 +257,24 @@ def test_captured_and_replayed(m, k, n):
         torch.cuda.synchronize()
         for a, c in zip(held, eager):
             assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """The last rows of results and residuals of more than 2^31 values are what they are by themselves."""
+    g = torch.Generator("cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=BF16)  # noqa: E731
+    m, k, n = 2 ** 22 + 77, 24, 520
+    x, w, b, res = r(m, k), r(n, k), r(n), r(m, n)
+    dy = r(m, n)
+    assert m * n > 2 ** 31
+    outs = []
+    for rows in (slice(None), slice(m - 1000, None)):
+        leaves = [x[rows].clone().requires_grad_(True), res[rows].clone().requires_grad_(True)]
+        y = linear_act(leaves[0], w, b, leaves[1], act="swish")
+        outs.append([t[-1000:] for t in (y.detach(), *torch.autograd.grad(y, leaves, dy[rows]))])
+        del y, leaves
+    # sums of 24 and of 520 terms in the same order of k: a step of bf16 where tiles differ
+    for a, c in zip(*outs):
+        assert torch.allclose(a.float(), c.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+
