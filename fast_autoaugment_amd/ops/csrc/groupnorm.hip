@@ -950,6 +950,9 @@ struct Whole { int tile, ntile, threads, r; };
 // read is cheaper, unless all workgroups run at once, when lines of 32 bytes do too. Measured (bf16, forward +
 // backward, us, whole/chunks): 128x14x14x1024 26+40/41+64, 128x28x28x512 41+98/62+104, 128x56x56x64 26+53/40+62,
 // 128x56x56x256 136+263/125+211.
+// Where a CU has two workgroups at most, their own waves have to hide what they wait for: 4 vectors a thread or
+// more threads (forward, us, against 8 or 16 vectors in 256): 128x32x32x32 10.9/11.5, 8x32x32x64 9.3/10.2,
+// 1x14x14x672 7.7/10.0; fewer than 4 gain nothing, 32x16x16x128 7.1 with 4 and 8.3 with 2.
 template <typename T, int VEC, int MOST_R>
 bool whole_of(const Shape& s, Whole& out) {
   const int64_t unit = std::lcm((int64_t)s.cg, (int64_t)VEC), line = sizeof(T) * unit;
@@ -969,8 +972,9 @@ bool whole_of(const Shape& s, Whole& out) {
   out.tile = (int)(k * unit);
   out.ntile = (int)((units + k - 1) / k);
   if (workgroups(k) >= (int64_t(1) << 22)) return false;
+  const int most_r = workgroups(k) <= 512 ? std::min(MOST_R, 4) : MOST_R;
   for (int threads : {256, 512, 1024})
-    for (out.r = 1; out.r <= MOST_R; out.r *= 2) {
+    for (out.r = 1; out.r <= (threads < 1024 ? most_r : MOST_R); out.r *= 2) {
       out.threads = (int)((((int64_t)s.S + out.r - 1) / out.r * (out.tile / VEC) + 63) / 64 * 64);
       if (out.threads <= threads) return true;
     }
