@@ -134,15 +134,12 @@ __device__ __forceinline__ float act_value(float z) {
   if (ACT == ACT_SIGMOID) return sigmoid(z);
   return z;
 }
-// d times the slope at z, or for relu at y: both are above 0 in the same places, but for z below half the type's
-// smallest number. Where relu holds back, no infinity or NaN of d comes through.
 template <int ACT>
-__device__ __forceinline__ float act_grad(float d, float z) {
-  if (ACT == ACT_RELU) return z <= 0.0f ? 0.0f : d;
+__device__ __forceinline__ float act_slope(float z) {
   const float s = sigmoid(z);
-  if (ACT == ACT_SWISH) return d * (s + s * (z - z * s));
-  if (ACT == ACT_SIGMOID) return d * (s - s * s);
-  return d;
+  if (ACT == ACT_SWISH) return s + s * (z - z * s);
+  if (ACT == ACT_SIGMOID) return s - s * s;
+  return 1.0f;
 }
 // f(activation as a constant): one branch outside the loops, not one an element
 template <bool ANY = true, typename F>
@@ -171,7 +168,8 @@ struct Epilogue {
   const T* bias;      // [N] or null
   const T* res;       // [M,N] or null
   T* y;               // [M,N]
-  T* z;               // [M,N] or null: the sum before the activation, for the backward pass
+  float* slope;       // [M,N] or null: the activation's slope, for the backward pass. It is made of the sum in 32 bits:
+                      // a sum held in 16 would be infinite beyond fp16's range, and cost the slope |z| 2^-9 in bf16
   int act;
   bool vec;           // rows of 4 (8 in 16 bits) may be read and written at once
 
@@ -183,7 +181,12 @@ struct Epilogue {
     const int64_t at = m * N + n;
     if (bias) v += load4(bias + n, left, vec);
     if (res) v += load4(res + at, left, vec);
-    if (z) store4(z + at, left, vec, v);
+    if (slope) {
+      f32x4 d;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = act_slope<ACT>(v[i]);
+      store4(slope + at, left, vec, d);
+    }
     #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(v[i]);
     store4(y + at, left, vec, v);
@@ -191,12 +194,14 @@ struct Epilogue {
   // 8 columns, 16 bytes at once; bias and residual are in v
   template <int ACT>
   __device__ __forceinline__ void eight(int64_t at, f32x8 v) const {
-    s16x8 out;
-    if (z) {
+    if (slope) {
+      f32x4 d[2];
       #pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = Num<T>::bits(v[e]);
-      *(s16x8*)(z + at) = out;
+      for (int e = 0; e < 8; ++e) d[e >> 2][e & 3] = act_slope<ACT>(v[e]);
+      *(f32x4*)(slope + at) = d[0];
+      *(f32x4*)(slope + at + 4) = d[1];
     }
+    s16x8 out;
     #pragma unroll
     for (int e = 0; e < 8; ++e) out[e] = Num<T>::bits(act_value<ACT>(v[e]));
     *(s16x8*)(y + at) = out;
@@ -646,9 +651,11 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // ------------------------------------------------------------ dz and its column sums
 
 // dz = dy act'(z), unless act is none; sums over a chunk of rows to part[chunk][N], or of all rows to db.
-// A thread has VEC columns, a workgroup a tile of columns and a chunk of rows.
+// A thread has VEC columns, a workgroup a tile of columns and a chunk of rows. `of` is what the slope is known from:
+// relu's result y, which is above 0 where z is, but for z below half the type's smallest number, or the slope itself.
+// Where relu holds back, no infinity or NaN of dy comes through.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const T* __restrict__ z,
+__global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const void* __restrict__ of,
                                                     T* __restrict__ dz, float* __restrict__ part, T* __restrict__ db,
                                                     int64_t M, int N, int tile, int ntile, int chunk,
                                                     int act) {
@@ -673,13 +680,19 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
         #pragma unroll
         for (int h = 0; h < H; ++h) d[h] = load4(dy + at + 4 * h, E, VEC > 1);
         if constexpr (A.value != ACT_NONE) {
-          f32x4 zz[H];
+          f32x4 s[H];
           #pragma unroll
-          for (int h = 0; h < H; ++h) zz[h] = load4(z + at + 4 * h, E, VEC > 1);
+          for (int h = 0; h < H; ++h) {
+            if constexpr (A.value == ACT_RELU) s[h] = load4((const T*)of + at + 4 * h, E, VEC > 1);
+            else s[h] = load4((const float*)of + at + 4 * h, E, VEC > 1);
+          }
           #pragma unroll
           for (int h = 0; h < H; ++h) {
             #pragma unroll
-            for (int i = 0; i < E; ++i) d[h][i] = act_grad<A.value>(d[h][i], zz[h][i]);
+            for (int i = 0; i < E; ++i) {
+              if constexpr (A.value == ACT_RELU) d[h][i] = s[h][i] <= 0.0f ? 0.0f : d[h][i];
+              else d[h][i] *= s[h][i];
+            }
             store4(dz + at + 4 * h, E, VEC > 1, d[h]);
           }
         }
@@ -769,7 +782,7 @@ template <typename T, bool PR, bool QR>
 void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hipStream_t stream) {
   const int64_t M = p.size(PR ? 1 : 0), N = q.size(QR ? 1 : 0), K = p.size(PR ? 0 : 1);
   constexpr int W = sizeof(T) == 2 ? 8 : 4;
-  epi.vec = N % W == 0 && aligned(epi.y, 16) && (!epi.z || aligned(epi.z, 16))
+  epi.vec = N % W == 0 && aligned(epi.y, 16) && (!epi.slope || aligned(epi.slope, 16))
             && (!epi.res || aligned(epi.res, 16)) && (!epi.bias || aligned(epi.bias, 16));
   int BM = 64, BN = 64, step = 16;
   if constexpr (sizeof(T) == 2) {
@@ -830,13 +843,13 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
 }
 
 template <typename T>
-void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, torch::Tensor* db, int act,
+void slope(const torch::Tensor& dy, const torch::Tensor* of, torch::Tensor* dz, torch::Tensor* db, int act,
            hipStream_t stream) {
   const int64_t M = dy.size(0);
   const int N = (int)dy.size(1);
   constexpr int V = 16 / sizeof(T);
   const bool vec = N % V == 0 && aligned(dy.data_ptr(), 16) && (!dz || (aligned(dz->data_ptr(), 16)
-                   && aligned(z->data_ptr(), 16)));
+                   && aligned(of->data_ptr(), 16)));
   const int vw = vec ? V : 1, tile = std::min(N, (vec ? 32 : 64) * vw), ntile = (N + tile - 1) / tile;
   const int rows = 256 / (tile / vw);
   // 1024 workgroups or more, as long as a thread has 4 rows (25088x256 takes 10 us, with fewer 16); few rows are
@@ -851,7 +864,7 @@ void slope(const torch::Tensor& dy, const torch::Tensor* z, torch::Tensor* dz, t
   if (join) ws = torch::empty({chunks * N}, dy.options().dtype(torch::kFloat32));
   auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((unsigned)(chunks * ntile)), dim3(256), 0, stream,
-                       (const T*)dy.data_ptr(), z ? (const T*)z->data_ptr() : nullptr,
+                       (const T*)dy.data_ptr(), of ? of->data_ptr() : nullptr,
                        dz ? (T*)dz->data_ptr() : nullptr, join ? ws.data_ptr<float>() : nullptr,
                        db && !join ? (T*)db->data_ptr() : nullptr, M, N, tile,
                        ntile, (int)chunk, act);
@@ -891,26 +904,26 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     auto stream = at::hip::getCurrentHIPStream().stream();
     auto y = torch::empty({x.size(0), w.size(0)}, x.options());
     const bool keep = train && (act == ACT_SWISH || act == ACT_SIGMOID);
-    auto z = keep ? torch::empty_like(y) : torch::Tensor();
+    auto slopes = keep ? torch::empty(y.sizes(), y.options().dtype(torch::kFloat32)) : torch::Tensor();
     if (x.size(0) > 0)
       by_type(x.scalar_type(), [&](auto t) {
         using T = decltype(t);
         Epilogue<T> epi{b.defined() ? (const T*)b.data_ptr() : nullptr,
                         r.defined() ? (const T*)r.data_ptr() : nullptr, (T*)y.data_ptr(),
-                        keep ? (T*)z.data_ptr() : nullptr, (int)act, false};
+                        keep ? slopes.data_ptr<float>() : nullptr, (int)act, false};
         product<T, false, false>(x, w, epi, stream);
       });
     C10_HIP_KERNEL_LAUNCH_CHECK();
     ctx->saved_data["how"] = act * 4 + b.defined() * 2 + r.defined();
     // relu's slope is known from its result
-    ctx->save_for_backward({x, w, keep ? z : act == ACT_RELU ? y : torch::Tensor()});
+    ctx->save_for_backward({x, w, keep ? slopes : act == ACT_RELU ? y : torch::Tensor()});
     return y;
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     auto saved = ctx->get_saved_variables();
-    const auto &x = saved[0], &w = saved[1], &z = saved[2];
+    const auto &x = saved[0], &w = saved[1], &of = saved[2];
     const int64_t how = ctx->saved_data["how"].toInt();
     const int act = (int)(how / 4);
     const c10::OptionalDeviceGuard guard(x.device());
@@ -936,7 +949,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
         by_type(x.scalar_type(), [&](auto t) {
           using T = decltype(t);
           if (act != ACT_NONE || nb)
-            slope<T>(dy, act == ACT_NONE ? nullptr : &z, act == ACT_NONE ? nullptr : &dz,
+            slope<T>(dy, act == ACT_NONE ? nullptr : &of, act == ACT_NONE ? nullptr : &dz,
                      nb ? &db : nullptr, act, stream);
           Epilogue<T> epi{nullptr, nullptr, nullptr, nullptr, ACT_NONE, false};
           if (nx) {

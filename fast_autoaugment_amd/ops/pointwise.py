@@ -42,9 +42,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     x is [..., K], weight [N, K], bias [N] and residual [..., N], all of one type
     (fp32, bf16 or fp16). ``act`` is "none", "relu", "swish" or "sigmoid". Sums
     are in fp32 and the result is rounded once. Gradients go to all four, once;
-    for swish and sigmoid the backward pass has the sum before the activation in
-    x's type, and for 16-bit types the products there take the gradient behind
-    the activation in that type too.
+    for swish and sigmoid the slopes are kept for them in fp32. For 16-bit types
+    the backward products take the gradient behind the activation in that type.
     """
     _check(x, weight, bias, residual, act)
     C = require_ext_for(x)

@@ -278,3 +278,43 @@ def test_offsets_beyond_32_bits():
     for a, c in zip(*outs):
         assert torch.allclose(a.float(), c.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
 
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act", ["swish", "sigmoid"])
+@pytest.mark.parametrize("m,k,n", [(40, 16, 24), (300, 8, 33), (3000, 24, 256), (131, 4000, 72)])
+def test_sums_beyond_fp16_have_their_slopes(dev, act, m, k, n):
+    """A sum of -120000 has no slope, one of 120000 swish's 1 and sigmoid's 0, though neither is a number of fp16. The
+    sums are exact and every slope is 0 or 1, so that gradients are those of the rows that have one, once rounded."""
+    x = torch.zeros(m, k, dtype=FP16)
+    x[:, 0] = torch.tensor([60000.0, -60000.0])[torch.arange(m) % 2]
+    w = torch.zeros(n, k, dtype=FP16)
+    w[:, 0] = 2.0
+    b = torch.zeros(n, dtype=FP16)
+    dy = torch.randint(-3, 4, (m, n), generator=torch.Generator().manual_seed(1)).to(FP16)
+    leaves = [t.to(dev).requires_grad_(True) for t in (x, w, b, torch.zeros(m, n, dtype=FP16))]
+    y = linear_act(leaves[0], leaves[1], leaves[2], leaves[3], act=act)
+    dx, dw, db, dr = (t.cpu() for t in torch.autograd.grad(y, leaves, dy.to(dev)))
+    dz = dy * (torch.arange(m) % 2 == 0).view(-1, 1) if act == "swish" else torch.zeros_like(dy)
+    assert torch.equal(dr, dz)
+    assert torch.equal(dx[:, 0], (2 * dz.double().sum(1)).to(FP16)) and not dx[:, 1:].any()
+    assert torch.equal(db, dz.double().sum(0).to(FP16))
+    assert torch.equal(dw[:, 0], (60000 * dz.double().sum(0)).to(FP16)) and not dw[:, 1:].any()
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act", ["swish", "sigmoid"])
+@pytest.mark.parametrize("t", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,k,n", [(128, 1152, 48), (77, 40, 33), (3000, 24, 256), (131, 4000, 72)])
+def test_a_slope_is_that_of_the_sum_in_32_bits(dev, act, t, m, k, n):
+    """The residual's gradient is dy times the slope, rounded once: the sum behind the slope is off by its fp32 terms'
+    (K + 4) f and the exponential's 2 f |z|, the slope by 8 f of its own, and nothing else is in fewer bits."""
+    x, w, b, r, dy = inputs(m, k, n, t, seed=2)
+    o = oracle(x, w, b, r, act, dy)
+    leaves = [v.to(dev).requires_grad_(True) for v in (x, w, b, r)]
+    y = linear_act(leaves[0], leaves[1], leaves[2], leaves[3], act=act)
+    got, = torch.autograd.grad(y, leaves[3:], o["dy"].to(dev))
+    u, f = torch.finfo(t).eps / 2, 2.0 ** -24
+    off = o["dy64"].abs() * (o["bend"] * ((k + 4) * f * o["size"] + 2 * f * o["z"].abs()) + 8 * f)
+    # half of a type's smallest step besides, where a result is smaller than its smallest normal number
+    close(got, o["dz"], u * (o["dz"].abs() + off) + off + torch.finfo(t).tiny * u)
