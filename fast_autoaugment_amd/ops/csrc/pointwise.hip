@@ -69,6 +69,7 @@ template <> struct Num<__hip_bfloat16> {
     __hip_bfloat16 h = __float2bfloat16(v);
     return *(short*)&h;
   }
+  static constexpr float kSecond = 1.0f;      // see Operand::second
   static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -80,6 +81,7 @@ template <> struct Num<__half> {
   static __device__ __forceinline__ void put(T* p, float v) { *p = __float2half(v); }
   static __device__ __forceinline__ float of(short u) { return __half2float(__ushort_as_half((unsigned short)u)); }
   static __device__ __forceinline__ short bits(float v) { return (short)__half_as_ushort(__float2half(v)); }
+  static constexpr float kSecond = 2048.0f;   // what is left of a value with half a step of error: fp16 has its bits
   static __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -211,10 +213,13 @@ struct Epilogue {
 // ------------------------------------------------------------ operands
 
 // P(row, k): row-major with k contiguous, or (ROWS) k-major with rows contiguous. Lines start at 16 bytes.
+// An fp32 operand is the sum of two in 16 bits: itself rounded, and `second` bytes further what that left over, times
+// kSecond. The product of both terms is exact to 2^-16 (bf16) or 2^-22 (fp16) of every value, at twice the steps.
 struct Operand {
   const short* p;
   int rows, kdim;
   int64_t ld;         // a multiple of 8
+  int64_t second;
 };
 
 // A tile of B rows and 64 k in LDS, pieces of 16 bytes, one after another as lanes load them: which piece of
@@ -315,7 +320,8 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t wg, uint32_t n) {
 // ------------------------------------------------------------ the product in 16 bits
 
 // Operands with contiguous rows are those of the gradients, which have no bias, residual or activation.
-template <typename T, bool PR, bool QR, int BM, int BN>
+// TWO: P has two terms. What is left over goes first, then the sums are scaled back and the rounded values follow.
+template <typename T, bool PR, bool QR, int BM, int BN, bool TWO>
 __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, Epilogue<T> epi,
                                                       float* __restrict__ part, int tiles_m,
                                                       int tiles_n, int splits) {
@@ -333,7 +339,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
   const int M = P.rows, N = Q.rows;
-  const LP load_p(P, m0, tid);
+  LP load_p(P, m0, tid);
   const LQ load_q(Q, n0, tid);
 
   f32x4 acc[FM][FN];
@@ -381,25 +387,38 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
         res[i][j / 2] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, mine + j * 16 < N ? at : 0xffffffffu, 0, 0);
       }
   }
-  fill(s0, p0, q0);
-  fill(s0 + 1, p1, q1);
-  int s = s0;
-  for (; s + 2 < s1; s += 2) {
-    come();
-    multiply(p0, q0);
-    read();
-    fill(s + 2, p0, q0);
-    come();
-    multiply(p1, q1);
-    read();
-    fill(s + 3, p1, q1);
+  auto steps_of_k = [&] {
+    fill(s0, p0, q0);
+    fill(s0 + 1, p1, q1);
+    int s = s0;
+    for (; s + 2 < s1; s += 2) {
+      come();
+      multiply(p0, q0);
+      read();
+      fill(s + 2, p0, q0);
+      come();
+      multiply(p1, q1);
+      read();
+      fill(s + 3, p1, q1);
+    }
+    if (s < s1) {     // one or two steps are left; no others are asked for
+      come();
+      multiply(p0, q0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + 1 < s1) multiply(p1, q1);
+  };
+  if constexpr (TWO) {
+    load_p.base += P.second;
+    steps_of_k();
+    load_p.base -= P.second;
+    #pragma unroll
+    for (int i = 0; i < FM; ++i)
+      #pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] *= 1.0f / Num<T>::kSecond;
+    read();           // the buffers are filled again
   }
-  if (s < s1) {     // one or two steps are left; no others are asked for
-    come();
-    multiply(p0, q0);
-  }
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  if (s + 1 < s1) multiply(p1, q1);
+  steps_of_k();
 
   // lane: output row lane%16 of a fragment; of fragments j, j+1 columns (lane/16)*8 + 0..3 and + 4..7
   auto each = [&](auto f) {
@@ -445,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
 // Few outputs: 32 x 32 of them a workgroup, and its 4 waves take every fourth step of k each, with buffers of their
 // own and no barrier between them; their sums meet in LDS at the end. One launch where the large tiles would have
 // to be split over workgroups and joined.
-template <typename T, bool PR, bool QR>
+template <typename T, bool PR, bool QR, bool TWO>
 __global__ __launch_bounds__(256) void small_product_kernel(Operand P, Operand Q, Epilogue<T> epi, int tiles_n) {
   constexpr int B = 32;
   typedef Loader<B, PR, false, 64> LP;
@@ -455,7 +474,7 @@ __global__ __launch_bounds__(256) void small_product_kernel(Operand P, Operand Q
   const int m0 = (int)tm * B, n0 = (int)(blockIdx.x - tm * tiles_n) * B;
   const int steps = (P.kdim + BK - 1) / BK;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const LP load_p(P, m0, lane);
+  LP load_p(P, m0, lane);
   const LQ load_q(Q, n0, lane);
   f32x4 acc[2][2];
   #pragma unroll
@@ -482,19 +501,29 @@ __global__ __launch_bounds__(256) void small_product_kernel(Operand P, Operand Q
         for (int j = 0; j < 2; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
     }
   };
-  fill(wave, p0[wave], q0[wave]);
-  fill(wave + 4, p1[wave], q1[wave]);
-  for (int s = wave; s < steps; s += 8) {
-    come();
-    multiply(p0[wave], q0[wave]);
-    read();
-    fill(s + 8, p0[wave], q0[wave]);
-    come();
-    multiply(p1[wave], q1[wave]);       // zeros where the step is not there
-    read();
-    fill(s + 12, p1[wave], q1[wave]);
+  auto steps_of_k = [&] {
+    fill(wave, p0[wave], q0[wave]);
+    fill(wave + 4, p1[wave], q1[wave]);
+    for (int s = wave; s < steps; s += 8) {
+      come();
+      multiply(p0[wave], q0[wave]);
+      read();
+      fill(s + 8, p0[wave], q0[wave]);
+      come();
+      multiply(p1[wave], q1[wave]);       // zeros where the step is not there
+      read();
+      fill(s + 12, p1[wave], q1[wave]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  if constexpr (TWO) {      // see product_kernel
+    load_p.base += P.second;
+    steps_of_k();
+    load_p.base -= P.second;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] *= 1.0f / Num<T>::kSecond;
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  steps_of_k();
   __syncthreads();
   // the waves' sums, 32 lines of 32 and 4 more (a line's start moves by 4 banks)
   constexpr int LD = B + 4;
@@ -653,10 +682,12 @@ __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ par
 // dz = dy act'(z), unless act is none; sums over a chunk of rows to part[chunk][N], or of all rows to db.
 // A thread has VEC columns, a workgroup a tile of columns and a chunk of rows. `of` is what the slope is known from:
 // relu's result y, which is above 0 where z is, but for z below half the type's smallest number, or the slope itself.
-// Where relu holds back, no infinity or NaN of dy comes through.
+// Where relu holds back, no infinity or NaN of dy comes through. `left` (or null) is given what dz's rounding left over,
+// times kSecond (see Operand): none where dz is infinite.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, const void* __restrict__ of,
-                                                    T* __restrict__ dz, float* __restrict__ part, T* __restrict__ db,
+                                                    T* __restrict__ dz, T* __restrict__ left,
+                                                    float* __restrict__ part, T* __restrict__ db,
                                                     int64_t M, int N, int tile, int ntile, int chunk,
                                                     int act) {
   __shared__ float lds[256 * VEC];
@@ -693,7 +724,29 @@ __global__ __launch_bounds__(256) void slope_kernel(const T* __restrict__ dy, co
               if constexpr (A.value == ACT_RELU) d[h][i] = s[h][i] <= 0.0f ? 0.0f : d[h][i];
               else d[h][i] *= s[h][i];
             }
+            if constexpr (std::is_same<T, __half>::value && A.value != ACT_RELU) {
+              // fp16 has an instruction that rounds a product at once: were it taken for one of dz's two uses below,
+              // what is left over would be that of another number than the one that is stored
+              #pragma unroll
+              for (int i = 0; i < E; ++i) {
+                float one = d[h][i];
+                asm("" : "+v"(one));
+                d[h][i] = one;
+              }
+            }
             store4(dz + at + 4 * h, E, VEC > 1, d[h]);
+            if constexpr (sizeof(T) == 2) {
+              if constexpr (A.value != ACT_RELU)
+                if (left) {
+                  f32x4 l;
+                  #pragma unroll
+                  for (int i = 0; i < E; ++i) {
+                    const float held = Num<T>::of(Num<T>::bits(d[h][i]));
+                    l[i] = __builtin_isinf(held) ? 0.0f : (d[h][i] - held) * Num<T>::kSecond;
+                  }
+                  store4(left + at + 4 * h, E, VEC > 1, l);
+                }
+            }
           }
         }
         #pragma unroll
@@ -756,6 +809,7 @@ void by_type(torch::ScalarType t, F f) {
 // t as an operand; `keep` holds a copy with wider lines where t's do not start at 16 bytes
 Operand operand(const torch::Tensor& t, bool rows_contiguous, torch::Tensor& keep, hipStream_t stream) {
   Operand o;
+  o.second = 0;
   o.rows = (int)t.size(rows_contiguous ? 1 : 0);
   o.kdim = (int)t.size(rows_contiguous ? 0 : 1);
   o.ld = t.size(1);
@@ -772,14 +826,21 @@ Operand operand(const torch::Tensor& t, bool rows_contiguous, torch::Tensor& kee
   return o;
 }
 
+// lines of both are equally wide: of one copy or none each, as both start at 16 bytes or neither does
+int64_t bytes_between(const Operand& a, const Operand& b) {
+  TORCH_CHECK(a.ld == b.ld && a.rows == b.rows && a.kdim == b.kdim, "linear_act: an operand's terms differ in shape");
+  return (const char*)b.p - (const char*)a.p;
+}
+
 OperandF32 operand_f32(const torch::Tensor& t, bool rows_contiguous) {
   return {t.data_ptr<float>(), (int)t.size(rows_contiguous ? 1 : 0), (int)t.size(rows_contiguous ? 0 : 1),
           t.size(1)};
 }
 
-// D[m][n] = sum_k P(m,k) Q(n,k), with the epilogue
-template <typename T, bool PR, bool QR>
-void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hipStream_t stream) {
+// D[m][n] = sum_k P(m,k) Q(n,k), with the epilogue. TWO: P is p + p_left / kSecond
+template <typename T, bool PR, bool QR, bool TWO = false>
+void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hipStream_t stream,
+             const torch::Tensor* p_left = nullptr) {
   const int64_t M = p.size(PR ? 1 : 0), N = q.size(QR ? 1 : 0), K = p.size(PR ? 0 : 1);
   constexpr int W = sizeof(T) == 2 ? 8 : 4;
   epi.vec = N % W == 0 && aligned(epi.y, 16) && (!epi.slope || aligned(epi.slope, 16))
@@ -808,9 +869,11 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
     // but 2048x1280x1000 (2048 tiles) 31/12, k = 6272 for 128x512 17/10, and k = 320 for 512x1280 (640) 7.8/3.9.
     const int64_t sm = (M + 31) / 32, sn = (N + 31) / 32;
     if (tm * tn < 256 && sm * sn <= 512 && steps >= 4 && steps <= 40) {
-      torch::Tensor keep_p, keep_q;
-      const Operand P = operand(p, PR, keep_p, stream), Q = operand(q, QR, keep_q, stream);
-      hipLaunchKernelGGL((small_product_kernel<T, PR, QR>), dim3((unsigned)(sm * sn)), dim3(256), 0, stream, P, Q,
+      torch::Tensor keep_p, keep_q, keep_left;
+      Operand P = operand(p, PR, keep_p, stream);
+      const Operand Q = operand(q, QR, keep_q, stream);
+      if constexpr (TWO) P.second = bytes_between(P, operand(*p_left, PR, keep_left, stream));
+      hipLaunchKernelGGL((small_product_kernel<T, PR, QR, TWO>), dim3((unsigned)(sm * sn)), dim3(256), 0, stream, P, Q,
                          epi, (int)sn);
       return;
     }
@@ -826,14 +889,16 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
     hipLaunchKernelGGL((product_f32_kernel<PR, QR>), grid, block, 0, stream, operand_f32(p, PR),
                        operand_f32(q, QR), epi, part, (int)tm, (int)tn, (int)splits);
   } else {
-    torch::Tensor keep_p, keep_q;
-    const Operand P = operand(p, PR, keep_p, stream), Q = operand(q, QR, keep_q, stream);
+    torch::Tensor keep_p, keep_q, keep_left;
+    Operand P = operand(p, PR, keep_p, stream);
+    const Operand Q = operand(q, QR, keep_q, stream);
+    if constexpr (TWO) P.second = bytes_between(P, operand(*p_left, PR, keep_left, stream));
     auto go = [&](auto kern) {
       hipLaunchKernelGGL(kern, grid, block, 0, stream, P, Q, epi, part, (int)tm, (int)tn, (int)splits);
     };
-    if (BM == 128 && BN == 128) go(product_kernel<T, PR, QR, 128, 128>);
-    else if (BM == 128) go(product_kernel<T, PR, QR, 128, 64>);
-    else go(product_kernel<T, PR, QR, 64, 64>);
+    if (BM == 128 && BN == 128) go(product_kernel<T, PR, QR, 128, 128, TWO>);
+    else if (BM == 128) go(product_kernel<T, PR, QR, 128, 64, TWO>);
+    else go(product_kernel<T, PR, QR, 64, 64, TWO>);
   }
   if (splits > 1) {
     const int64_t work = M * ((N + 3) / 4);
@@ -843,13 +908,13 @@ void product(const torch::Tensor& p, const torch::Tensor& q, Epilogue<T> epi, hi
 }
 
 template <typename T>
-void slope(const torch::Tensor& dy, const torch::Tensor* of, torch::Tensor* dz, torch::Tensor* db, int act,
-           hipStream_t stream) {
+void slope(const torch::Tensor& dy, const torch::Tensor* of, torch::Tensor* dz, torch::Tensor* left,
+           torch::Tensor* db, int act, hipStream_t stream) {
   const int64_t M = dy.size(0);
   const int N = (int)dy.size(1);
   constexpr int V = 16 / sizeof(T);
   const bool vec = N % V == 0 && aligned(dy.data_ptr(), 16) && (!dz || (aligned(dz->data_ptr(), 16)
-                   && aligned(of->data_ptr(), 16)));
+                   && aligned(of->data_ptr(), 16))) && (!left || aligned(left->data_ptr(), 16));
   const int vw = vec ? V : 1, tile = std::min(N, (vec ? 32 : 64) * vw), ntile = (N + tile - 1) / tile;
   const int rows = 256 / (tile / vw);
   // 1024 workgroups or more, as long as a thread has 4 rows (25088x256 takes 10 us, with fewer 16); few rows are
@@ -865,7 +930,7 @@ void slope(const torch::Tensor& dy, const torch::Tensor* of, torch::Tensor* dz, 
   auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((unsigned)(chunks * ntile)), dim3(256), 0, stream,
                        (const T*)dy.data_ptr(), of ? of->data_ptr() : nullptr,
-                       dz ? (T*)dz->data_ptr() : nullptr, join ? ws.data_ptr<float>() : nullptr,
+                       dz ? (T*)dz->data_ptr() : nullptr, left ? (T*)left->data_ptr() : nullptr, join ? ws.data_ptr<float>() : nullptr,
                        db && !join ? (T*)db->data_ptr() : nullptr, M, N, tile,
                        ntile, (int)chunk, act);
   };
@@ -932,7 +997,7 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
     const bool has_b = how & 2, has_r = how & 1;
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1),
                nb = has_b && ctx->needs_input_grad(2), nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
-    torch::Tensor dy, dz, dx, dw, db;
+    torch::Tensor dy, dz, left, dx, dw, db;
     const int64_t M = x.size(0), N = w.size(0);
     const bool again = at::GradMode::is_enabled();
     {
@@ -942,6 +1007,10 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
       if (nx) dx = torch::empty_like(x);
       if (nw) dw = torch::empty_like(w);
       dz = act == ACT_NONE ? dy : torch::empty_like(dy);
+      // The slopes of swish and sigmoid make dz a number of 32 bits, which one of 16 cannot hold for the products: a
+      // gradient's error in bf16 would be 1.4 times that of its own rounding. Others' dz is dy or 0.
+      const bool two = (act == ACT_SWISH || act == ACT_SIGMOID) && dy.element_size() == 2 && (nx || nw);
+      if (two) left = torch::empty_like(dy);
       if (M == 0) {
         if (nb) db.zero_();
         if (nw) dw.zero_();
@@ -949,17 +1018,22 @@ class LinearAct : public torch::autograd::Function<LinearAct> {
         by_type(x.scalar_type(), [&](auto t) {
           using T = decltype(t);
           if (act != ACT_NONE || nb)
-            slope<T>(dy, act == ACT_NONE ? nullptr : &of, act == ACT_NONE ? nullptr : &dz,
+            slope<T>(dy, act == ACT_NONE ? nullptr : &of, act == ACT_NONE ? nullptr : &dz, two ? &left : nullptr,
                      nb ? &db : nullptr, act, stream);
           Epilogue<T> epi{nullptr, nullptr, nullptr, nullptr, ACT_NONE, false};
-          if (nx) {
-            epi.y = (T*)dx.data_ptr();
-            product<T, false, true>(dz, w, epi, stream);
-          }
-          if (nw) {
-            epi.y = (T*)dw.data_ptr();
-            product<T, true, true>(dz, x, epi, stream);
-          }
+          auto products = [&](auto terms) {
+            if (nx) {
+              epi.y = (T*)dx.data_ptr();
+              product<T, false, true, terms.value>(dz, w, epi, stream, &left);
+            }
+            if (nw) {
+              epi.y = (T*)dw.data_ptr();
+              product<T, true, true, terms.value>(dz, x, epi, stream, &left);
+            }
+          };
+          if constexpr (sizeof(T) == 2)
+            if (two) return products(std::true_type{});
+          products(std::false_type{});
         });
         C10_HIP_KERNEL_LAUNCH_CHECK();
       }

@@ -42,8 +42,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     x is [..., K], weight [N, K], bias [N] and residual [..., N], all of one type
     (fp32, bf16 or fp16). ``act`` is "none", "relu", "swish" or "sigmoid". Sums
     are in fp32 and the result is rounded once. Gradients go to all four, once;
-    for swish and sigmoid the slopes are kept for them in fp32. For 16-bit types
-    the backward products take the gradient behind the activation in that type.
+    for swish and sigmoid the slopes are kept for them in fp32, and for 16-bit
+    types the backward products take the gradient behind the activation as a sum
+    of two numbers of that type, which holds 16 (bf16) or 22 (fp16) bits of it.
     """
     _check(x, weight, bias, residual, act)
     C = require_ext_for(x)

@@ -318,3 +318,61 @@ def test_a_slope_is_that_of_the_sum_in_32_bits(dev, act, t, m, k, n):
     off = o["dy64"].abs() * (o["bend"] * ((k + 4) * f * o["size"] + 2 * f * o["z"].abs()) + 8 * f)
     # half of a type's smallest step besides, where a result is smaller than its smallest normal number
     close(got, o["dz"], u * (o["dz"].abs() + off) + off + torch.finfo(t).tiny * u)
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act", ["swish", "sigmoid"])
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -17])
+@pytest.mark.parametrize("m,k,n", [(128, 1152, 48), (100, 48, 1152), (77, 40, 33), (3000, 24, 256), (2500, 264, 136),
+                                   (131, 4000, 72), (33, 520, 2047)])
+def test_products_have_the_gradient_behind_the_activation_to_more_than_the_type(dev, act, t, scale, m, k, n):
+    """dz, made of fp32 slopes (see above), is held as two numbers of the type: half a step u of the first, whose
+    own error is u of that again, or half a smallest step where that is more (2^-25 in fp16, and there the second is
+    held times 2048: 2^-36). Products carry that, their fp32 sums (2 and 4 more terms of N or M, both passes) and one
+    rounding."""
+    x, w, b, r, dy = inputs(m, k, n, t, seed=3)
+    o = oracle(x, w, b, r, act, (dy.float() * scale).to(t))
+    leaves = [v.to(dev).requires_grad_(True) for v in (x, w, b)]
+    y = linear_act(leaves[0], leaves[1], leaves[2], r.to(dev), act=act)
+    dx, dw, _ = torch.autograd.grad(y, leaves, o["dy"].to(dev))
+    u, f = torch.finfo(t).eps / 2, 2.0 ** -24
+    off = o["dy64"].abs() * (o["bend"] * ((k + 4) * f * o["size"] + 2 * f * o["z"].abs()) + 8 * f)
+    off = off + u * u * o["dz"].abs() + (2.0 ** -36 if t == FP16 else 2.0 ** -133)
+    least = torch.finfo(t).tiny * u
+    dz, ax, aw = o["dz"].abs(), o["x"].abs(), o["w"].abs()
+    tol_x, tol_w = off @ aw + (2 * n + 4) * f * (dz @ aw), off.t() @ ax + (2 * m + 4) * f * (dz.t() @ ax)
+    close(dx, o["dx"], u * (o["dx"].abs() + tol_x) + tol_x + least)
+    close(dw, o["dw"], u * (o["dw"].abs() + tol_w) + tol_w + least)
+    # what a dz rounded once gives would not pass where sums are short: the share of long ones grows with their length
+    if n < 64 and t == BF16 and scale == 1.0:
+        once = o["dz"].to(t).double() @ o["w"]
+        assert (once.to(t).double() - o["dx"]).abs().gt(u * (o["dx"].abs() + tol_x) + tol_x + least).any()
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act", ["swish", "sigmoid"])
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("m,k,n", [(60, 16, 24), (300, 72, 33), (3000, 24, 256), (131, 4000, 72)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_gradient_that_is_no_number_stays_in_its_row_and_column(dev, act, t, m, k, n, bad):
+    x, w, b, r, dy = inputs(m, k, n, t, seed=4)
+    x, w = (torch.where(v == 0, torch.ones_like(v), v) for v in (x, w))       # 0 times infinity is no infinity
+    grads = []
+    for value in (1.0, bad):
+        dy[7, 5] = value
+        leaves = [v.to(dev).requires_grad_(True) for v in (x, w, b, r)]
+        y = linear_act(*leaves[:3], residual=leaves[3], act=act)
+        grads.append([g.cpu() for g in torch.autograd.grad(y, leaves, dy.to(dev))])
+    (dx0, dw0, db0, dr0), (dx, dw, db, dr) = grads
+    z = x[7].double() @ w[5].double() + b[5].double() + r[7, 5].double()
+    sig = torch.sigmoid(z)
+    want = torch.tensor(bad) * (sig * (1 + z * (1 - sig)) if act == "swish" else 1)
+    for got, value in ((dx[7], want * w[5].double()), (dw[5], want * x[7].double()), (db[5], want), (dr[7, 5], want)):
+        assert torch.equal(torch.isnan(got), torch.isnan(value).expand(got.shape)), "NaN"
+        if not math.isnan(bad):
+            assert torch.equal(got.double(), value)
+    rows, cols = torch.arange(m) != 7, torch.arange(n) != 5
+    assert torch.equal(dx[rows], dx0[rows]) and torch.equal(dw[cols], dw0[cols]) and torch.equal(db[cols], db0[cols])
+    dr[7, 5] = dr0[7, 5]
+    assert torch.equal(dr, dr0)
