@@ -268,9 +268,9 @@ class FusedAdamW:
     fp32, bf16 or fp16, and all on one device; bf16 and fp16 ones get fp32
     weights that the optimizer keeps (FlatParams brings its own), which are
     updated and rounded back into the parameters. Such a parameter that was
-    written since the last step (a checkpoint that was loaded) is taken over
-    where it is not its fp32 weight rounded; a write through ``p.data`` is not
-    seen. A parameter whose ``grad`` is None is left as it is. The step count is one for all parameters.
+    written since the last step (a checkpoint that was loaded), or a flat buffer
+    or one of its parameters, is taken over where it is not its fp32 weight
+    rounded; a write through ``p.data`` is not seen. A parameter whose ``grad`` is None is left as it is. The step count is one for all parameters.
 
     ``state_bits=8`` holds m and sqrt(v) as e4m3 numbers (``exp_avg``,
     ``exp_avg_root``) with one fp32 scale for every 256 neighbours of a tensor
@@ -281,7 +281,8 @@ class FusedAdamW:
 
     The step count and the learning rate are on the device: a captured step
     replays, with ``sync_lr()`` before a replay pushing a changed rate. Under
-    capture the gradients have to be where an eager step saw them.
+    capture the gradients have to be where an eager step saw them. Weights that
+    were written between replays are not seen by these: an eager step comes first.
     """
 
     BLOCK = 256         # elements under one scale
@@ -344,6 +345,7 @@ class FusedAdamW:
                              "256 in the flat buffer: flatten_module(align=256)")
         self._dev = f.flat_param.device
         self._items = [(0, nd, self.weight_decay), (nd, n - nd, 0.0)]
+        self._flat_stamp = None
         return n
 
     def _init_list(self, params):
@@ -383,6 +385,21 @@ class FusedAdamW:
     def _stamp(p):
         """What changes when a tensor is written by torch or put elsewhere."""
         return p.data_ptr(), 0 if p.is_inference() else p._version
+
+    def _take_over_flat(self):
+        """Weights that were written into low-precision flat buffers since the last step go to the fp32 ones."""
+        f = self.flat
+        if f.flat_param.dtype == torch.float32:
+            return
+        # a parameter of the buffer counts its own writes
+        stamp = (*self._stamp(f.flat_param), sum(self._stamp(p)[1] for p in f.params))
+        if stamp == self._flat_stamp:
+            return
+        if self._dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: the flat weights were written since the last eager step: step once before capture")
+        full, low = f.flat_master, f.flat_param
+        full.copy_(torch.where(full.to(low.dtype) == low, full, low.float()))
+        self._flat_stamp = stamp
 
     @staticmethod
     def _same_order(a, b):
@@ -482,6 +499,8 @@ class FusedAdamW:
     @torch.no_grad()
     def step(self):
         self.lr = self.param_groups[0]["lr"]
+        if self.flat is not None:
+            self._take_over_flat()
         if self._dev.type != "cuda":
             return self._step_cpu()
         from .ops import ext
@@ -549,6 +568,8 @@ class FusedAdamW:
             self._hold(second, off, n, v if self.state_bits == 32 else root, True)
         if self.flat is None:
             self._stamps = [self._stamp(p) for p in self.params]
+        elif self._flat_stamp is not None:
+            self._flat_stamp = (*self._stamp(self.flat.flat_param), self._flat_stamp[-1])
 
     def state_dict(self):
         sd = {"step": int(self.step_count), "lr": self.lr, "state_bits": self.state_bits}

@@ -454,3 +454,83 @@ def test_offsets_beyond_32_bits(bits):
     for a, b in zip(*got):
         assert torch.equal(a, b)
 
+
+
+def flat_model(dev, dtype, seed=0):
+    torch.manual_seed(seed)
+    model = nn.Sequential(nn.Conv2d(3, 7, 3), nn.BatchNorm2d(7), nn.Flatten(), nn.Linear(63, 11)).to(dev)
+    return model, flatten_module(model, align=256, work_dtype=dtype)
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("how", ["model", "buffer", "before"])
+def test_flat_weights_that_were_loaded_are_taken_over(dev, bits, dtype, how):
+    """As those of lists: through the model or the buffer, and those that were loaded before the first step."""
+    model, flat = flat_model(dev, dtype)
+    opt = FusedAdamW(flat, lr=1e-3, state_bits=bits)
+
+    def load(value):
+        if how == "buffer":
+            with torch.no_grad():
+                flat.flat_param.fill_(value)
+        else:
+            model.load_state_dict({k: torch.full_like(v, value) for k, v in model.state_dict().items()})
+
+    for step in range(1 if how == "before" else 3):
+        if how != "before":
+            flat.flat_grad.fill_(1.0)
+            opt.step()
+        held = flat.flat_master.clone()
+        load(3.0)
+        opt.param_groups[0]["lr"] = 0.0
+        flat.flat_grad.fill_(1.0)
+        opt.step()
+        # a step of lr 1e-3 from 3 still rounds to 3 in bf16 (its numbers lie 2^-6 apart there), and is kept
+        for p in flat.params:
+            at = (p.data_ptr() - flat.flat_param.data_ptr()) // p.element_size()
+            mine, before = (t[at:at + p.numel()] for t in (flat.flat_master, held))
+            assert torch.equal(mine, torch.where(before.to(dtype) == 3.0, before, 3.0)) and (p.detach() == 3.0).all()
+        opt.param_groups[0]["lr"] = 1e-3
+
+
+@pytest.mark.parametrize("dev", DEV)
+def test_flat_weights_that_the_step_wrote_keep_their_fp32_digits(dev):
+    model, flat = flat_model(dev, torch.bfloat16)
+    opt = FusedAdamW(flat, lr=1e-3)
+    for step in range(3):
+        flat.flat_grad.fill_(1.0)
+        opt.step()
+    assert not torch.equal(flat.flat_master, flat.flat_param.float())
+    held = flat.flat_master.clone()
+    with torch.no_grad():
+        for p in flat.params:
+            p.copy_(p.clone())            # written, and nothing changed
+    opt.param_groups[0]["lr"] = 0.0
+    opt.step()
+    assert torch.equal(flat.flat_master, held)
+
+
+@pytest.mark.gpu
+def test_a_capture_refuses_flat_weights_that_were_written():
+    model, flat = flat_model("cuda", torch.bfloat16)
+    opt = FusedAdamW(flat, lr=1e-3)
+    opt.step()
+    with torch.no_grad():
+        flat.flat_param.fill_(1.0)
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    graph = torch.cuda.CUDAGraph()
+    opt.step()          # an eager one takes them over, and the next is captured
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    flat.flat_grad.fill_(1.0)
+    before = flat.flat_master.clone()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not torch.equal(flat.flat_master, before)
+        before = flat.flat_master.clone()
