@@ -576,6 +576,8 @@ class FusedAdamW:
         sd.update({n: getattr(self, n) for n in self._names})
         if self.flat is None and any(m is not None for m in self.masters):
             sd["masters"] = self.masters
+        elif self.flat is not None and self.flat.flat_param.dtype != torch.float32:
+            sd["flat_master"] = self.flat.flat_master
         return sd
 
     @torch.no_grad()
@@ -588,8 +590,13 @@ class FusedAdamW:
         for n in self._names:
             if sd[n].shape != getattr(self, n).shape or sd[n].dtype != getattr(self, n).dtype:
                 raise ValueError(f"FusedAdamW: {n} has another shape or type than this optimizer's")
+        low = self.flat is not None and self.flat.flat_param.dtype != torch.float32
+        if low and "flat_master" in sd and sd["flat_master"].shape != self.flat.flat_master.shape:
+            raise ValueError("FusedAdamW: flat_master has another shape than this optimizer's")
         for n in self._names:
             getattr(self, n).copy_(sd[n])
+        if low and "flat_master" in sd:
+            self.flat.flat_master.copy_(sd["flat_master"])
         if self.flat is None and "masters" in sd:
             for mine, theirs in zip(self.masters, sd["masters"]):
                 if mine is not None:

@@ -534,3 +534,49 @@ def test_a_capture_refuses_flat_weights_that_were_written():
         torch.cuda.synchronize()
         assert not torch.equal(flat.flat_master, before)
         before = flat.flat_master.clone()
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("order", ["weights first", "state first"])
+def test_flat_state_survives_saving(dev, bits, dtype, order, tmp_path):
+    """A run that was saved with its weights as the trainer saves them goes on bit by bit."""
+    def go(flat, opt, steps):
+        for step in steps:
+            g = torch.Generator().manual_seed(step)
+            for p in flat.params:
+                p.grad.copy_(torch.randn(p.shape, generator=g))
+            opt.step()
+
+    make = lambda seed: (lambda m: (*m, FusedAdamW(m[1], lr=1e-3, weight_decay=0.1, state_bits=bits)))(  # noqa: E731
+        flat_model(dev, dtype, seed))
+    _, flat_a, opt_a = make(0)
+    go(flat_a, opt_a, range(4))
+    model, flat_b, opt_b = make(0)
+    go(flat_b, opt_b, range(2))
+    torch.save({"opt": opt_b.state_dict(), "model": {k: v.float() for k, v in model.state_dict().items()}}, tmp_path / "s.pth")
+    sd = torch.load(tmp_path / "s.pth", weights_only=True)
+    model, flat_c, opt_c = make(1)
+    if order == "state first":
+        opt_c.load_state_dict(sd["opt"])
+    model.load_state_dict(sd["model"])
+    if dtype != torch.float32:
+        flat_c.flat_master.copy_(flat_c.flat_param) if order == "weights first" else None
+    if order == "weights first":
+        opt_c.load_state_dict(sd["opt"])
+    go(flat_c, opt_c, range(2, 4))
+    full = lambda f: f.flat_param if f.flat_master is None else f.flat_master  # noqa: E731
+    assert torch.equal(full(flat_a), full(flat_c)) and torch.equal(flat_a.flat_param, flat_c.flat_param)
+    for n in opt_a._names:
+        assert torch.equal(getattr(opt_a, n).float(), getattr(opt_c, n).float())
+
+
+def test_a_state_of_other_weights_is_refused():
+    _, flat = flat_model("cpu", torch.bfloat16)
+    opt = FusedAdamW(flat)
+    sd = opt.state_dict()
+    before = opt.exp_avg.fill_(0.5).clone()
+    with pytest.raises(ValueError):
+        opt.load_state_dict({**sd, "exp_avg": torch.zeros_like(before), "flat_master": torch.zeros(3)})
+    assert torch.equal(opt.exp_avg, before)
