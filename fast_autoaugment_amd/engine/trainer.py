@@ -365,6 +365,11 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
 
     result = OrderedDict()
     epoch_start = 1
+    def weights_were_loaded():
+        """The flat optimizers step from their fp32 weights: they take over what was loaded into the model."""
+        if use_fast:
+            flat.flat_master.copy_(flat.flat_param)
+
     # checkpoint load + resume (reference train.py:191-218)
     if save_path != "test.pth" and save_path and os.path.exists(save_path):
         logger.info("%s found. loading...", save_path)
@@ -372,13 +377,13 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
         key = "model" if "model" in data else "state_dict"
         if "epoch" not in data:
             model.load_state_dict(data)
+            weights_were_loaded()
         else:
             logger.info("checkpoint epoch@%d", data["epoch"])
             sd = data[key]
             raw = model.module if hasattr(model, "module") else model
             raw.load_state_dict({k.replace("module.", ""): v for k, v in sd.items()})
-            if use_fast:
-                flat.flat_master.copy_(flat.flat_param.float())
+            weights_were_loaded()
             try:
                 optimizer.load_state_dict(data["optimizer"])
             except Exception as e:
@@ -472,6 +477,7 @@ def train_and_eval(tag, dataroot, test_ratio=0.0, cv_fold=0, reporter=None,
                 import torch.distributed as dist
                 for _, x in raw.state_dict().items():
                     dist.broadcast(x, 0)
+            weights_were_loaded()
 
         if is_master and (epoch % evaluation_interval == 0 or epoch == max_epoch):
             with torch.no_grad():

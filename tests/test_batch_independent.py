@@ -259,3 +259,50 @@ def test_a_child_of_another_norm_is_not_the_cached_one(tmp_path):
         model = _cached_model(conf, 10, path, "cpu")
         groups.add(max(m.num_groups for m in model.modules() if isinstance(m, torch.nn.GroupNorm)))
     assert groups == {8, 4}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("optimizer", [{"type": "sgd", "decay": 0.0}, {"type": "rmsprop", "decay": 0.0},
+                                       {"type": "adamw", "decay": 0.05}, {"type": "adamw", "decay": 0.05, "state_bits": 8}])
+@pytest.mark.parametrize("loaded", ["average", "bare checkpoint"])
+def test_the_trainer_steps_from_weights_that_were_loaded(optimizer, loaded, tmp_path, monkeypatch):
+    """An average that is copied into the model at an epoch's end, or a checkpoint of weights alone, is what the fp32
+    weights of the next epoch start from: those round to the model's, and the model's are what was loaded."""
+    monkeypatch.setenv("FAA_SYNTH_TRAIN", "64")
+    monkeypatch.setenv("FAA_SYNTH_TEST", "32")
+    from fast_autoaugment_amd.data import api as data_api
+    from fast_autoaugment_amd.engine import trainer
+    starts, run_epoch = [], trainer.run_epoch
+
+    def watched(model, loader, loss_fn, opt, *args, **kwargs):
+        if opt is not None:
+            flat = opt.flat
+            starts.append(({k: v.detach().clone() for k, v in model.state_dict().items()},
+                           torch.equal(flat.flat_master.bfloat16(), flat.flat_param)))
+        return run_epoch(model, loader, loss_fn, opt, *args, **kwargs)
+
+    monkeypatch.setattr(trainer, "run_epoch", watched)
+    averages, ema = [], trainer.EMA
+    monkeypatch.setattr(ema, "state_dict", lambda self: averages.append({k: v.clone() for k, v in self.shadow.items()})
+                        or {k: v.clone() for k, v in self.shadow.items()})
+    conf = {
+        "model": {"type": "wresnet40_2", "norm": "group"}, "dataset": "cifar10", "aug": "default", "cutout": 0,
+        "batch": 32, "epoch": 2, "lr": 0.05, "lr_schedule": {"type": "cosine", "warmup": {"multiplier": 1, "epoch": 0}},
+        "optimizer": {**optimizer, "clip": 5, "ema": 0.5 if loaded == "average" else 0, "ema_interval": 1},
+    }
+    path = None
+    if loaded != "average":
+        path = str(tmp_path / "weights.pth")
+        torch.manual_seed(123)
+        averages = [{k: v.float() for k, v in build_model(conf["model"], 10).state_dict().items()}]
+        torch.save(averages[0], path)
+    try:
+        data_api._STORE_CACHE.clear()
+        C.replace(conf)
+        trainer.train_and_eval("", "./data", save_path=path, evaluation_interval=5)
+    finally:
+        data_api._STORE_CACHE.clear()
+    weights, rounded = starts[1 if loaded == "average" else 0]
+    assert rounded
+    for k, v in averages[0].items():
+        assert torch.equal(weights[k].float().cpu(), v.to(weights[k].dtype).float().cpu())
