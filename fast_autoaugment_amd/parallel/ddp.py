@@ -44,6 +44,8 @@ class FlatDDP(nn.Module):
             # rank-0 weight broadcast (reference train.py:220-224) — one call
             # on the flat buffer + per-buffer broadcast for BN running stats
             dist.broadcast(self.flat.flat_param, 0, group=self.pg)
+            if self.flat.flat_master is not None:   # what the optimizers step from
+                dist.broadcast(self.flat.flat_master, 0, group=self.pg)
             for _, b in module.named_buffers():
                 dist.broadcast(b, 0, group=self.pg)
 

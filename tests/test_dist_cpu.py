@@ -294,3 +294,49 @@ def test_flatddp_world8_matches_single_process():
         loss.backward()
         opt.step()
     assert torch.allclose(flats[0], flat.flat_param, atol=1e-5)
+
+
+def _master_worker(rank, world, port, kind, results):
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    torch.manual_seed(70 + rank)
+    from fast_autoaugment_amd.optim import FusedAdamW, FusedRMSpropTF, FusedSGD
+    from fast_autoaugment_amd.parallel.ddp import FlatDDP
+    ddp = FlatDDP(torch.nn.Sequential(torch.nn.Linear(6, 9), torch.nn.ReLU(), torch.nn.Linear(9, 3)),
+                  work_dtype=torch.bfloat16, align=256)
+    first = ddp.flat.flat_master.clone()
+    make = {"sgd": lambda f: FusedSGD(f, lr=0.1), "rmsprop": lambda f: FusedRMSpropTF(f, lr=0.01),
+            "adamw": lambda f: FusedAdamW(f, lr=0.01, state_bits=8)}[kind]
+    opt = make(ddp.flat)
+    torch.manual_seed(7)
+    data = torch.randn(4 * world, 6).bfloat16()[rank::world]
+    for _ in range(2):
+        opt.zero_grad()
+        ddp(data).float().square().mean().backward()
+        ddp.finish_gradient_sync()
+        opt.step()
+    results[rank] = (first, ddp.flat.flat_master.clone(), ddp.flat.flat_param.float().clone())
+    dist.destroy_process_group()
+
+
+@pytest.mark.timeout(180)
+@pytest.mark.parametrize("kind", ["sgd", "rmsprop", "adamw"])
+def test_ranks_start_from_the_same_fp32_weights(kind):
+    """Ranks whose models began differently train the first one's: in bf16 that is its fp32 weights."""
+    port, ctx = _find_port(), mp.get_context("spawn")
+    with mp.Manager() as mgr:
+        results = mgr.dict()
+        procs = [ctx.Process(target=_master_worker, args=(r, 2, port, kind, results)) for r in range(2)]
+        for p in procs:
+            p.start()
+        for p in procs:
+            p.join(150)
+            assert p.exitcode == 0
+        (first, *rest), (theirs, *others) = results[0], results[1]
+    # the first rank's own weights, with the digits that bf16 has not
+    torch.manual_seed(70)
+    own = torch.nn.Linear(6, 9).weight.detach().flatten()
+    assert torch.equal(first[:54], own) and torch.equal(theirs, first)
+    for a, b in zip(rest, others):
+        assert torch.equal(a, b)
