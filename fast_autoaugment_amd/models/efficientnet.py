@@ -21,7 +21,7 @@ from torch.nn import functional as F
 
 from ..ops.functional import Swish, drop_connect
 from ..ops.modules import bn_only, bn_swish
-from ..ops.pointwise import linear_act
+from ..ops.pointwise import DTYPES, linear_act
 
 
 def _bn(bn, x):
@@ -223,7 +223,7 @@ class MBConvBlock(nn.Module):
         x = _bn_swish(self._bn1, conv(self._depthwise_conv, x), self._swish)
         if self.has_se:
             sq = F.adaptive_avg_pool2d(x, 1)
-            if self.fused_se and self._se_reduce.weight.dtype == sq.dtype:
+            if self.fused_se and self._se_reduce.weight.dtype == sq.dtype and sq.dtype in DTYPES:
                 gate = linear_act(sq.flatten(1), self._se_reduce.weight.flatten(1), self._se_reduce.bias, act="swish")
                 gate = linear_act(gate, self._se_expand.weight.flatten(1), self._se_expand.bias, act="sigmoid")
                 x = gate[:, :, None, None] * x

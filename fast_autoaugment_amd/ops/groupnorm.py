@@ -14,7 +14,7 @@ import torch.nn.functional as F
 from . import require_ext_for
 
 ACTS = {"none": 0, "relu": 1, "swish": 2}
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _check(x, num_groups, weight, bias, eps, act):
@@ -22,7 +22,7 @@ def _check(x, num_groups, weight, bias, eps, act):
         raise ValueError(f"group_norm_act: act={act!r} is none of {sorted(ACTS)}")
     if x.dim() < 2:
         raise ValueError("group_norm_act: x is [N, C, ...]")
-    if x.dtype not in _DTYPES:
+    if x.dtype not in DTYPES:
         raise TypeError(f"group_norm_act: x is fp32, bf16 or fp16, not {x.dtype}")
     c = x.size(1)
     if num_groups < 1 or c < 1 or c % num_groups:
@@ -77,9 +77,11 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
 
 
 class GroupNormAct(torch.nn.GroupNorm):
-    """nn.GroupNorm on ``group_norm_act``; ``ops.modules`` fuses the activation that follows it."""
+    """nn.GroupNorm on ``group_norm_act`` where that has x's type; ``ops.modules`` fuses the activation that follows it."""
 
     act = "none"
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dtype not in DTYPES:
+            return super().forward(x)
         return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act)

@@ -12,13 +12,13 @@ import torch
 from . import require_ext_for
 
 ACTS = {"none": 0, "relu": 1, "swish": 2, "sigmoid": 3}
-_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _check(x, weight, bias, residual, act):
     if act not in ACTS:
         raise ValueError(f"linear_act: act={act!r} is none of {sorted(ACTS)}")
-    if x.dtype not in _DTYPES:
+    if x.dtype not in DTYPES:
         raise TypeError(f"linear_act: x is fp32, bf16 or fp16, not {x.dtype}")
     if x.dim() < 1 or weight.dim() != 2 or x.size(-1) != weight.size(1):
         raise ValueError(f"linear_act: x [..., K] and weight [N, K], not {list(x.shape)} and {list(weight.shape)}")
@@ -89,7 +89,7 @@ class LinearAct(torch.nn.Linear):
     act = "none"
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.dtype != self.weight.dtype or x.dtype not in _DTYPES:
+        if x.dtype != self.weight.dtype or x.dtype not in DTYPES:
             return torch.nn.functional.linear(x, self.weight, self.bias)
         return linear_act(x, self.weight, self.bias, act=self.act)
 

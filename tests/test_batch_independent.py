@@ -306,3 +306,27 @@ def test_the_trainer_steps_from_weights_that_were_loaded(optimizer, loaded, tmp_
     assert rounded
     for k, v in averages[0].items():
         assert torch.equal(weights[k].float().cpu(), v.to(weights[k].dtype).float().cpu())
+
+
+@pytest.mark.parametrize("call,after", [("bn_relu", torch.relu), ("bn_only", lambda t: t), ("bn_swish", nn.functional.silu)])
+def test_group_norms_in_fp64_run_as_torch_s(call, after):
+    from fast_autoaugment_amd.ops import modules
+    torch.manual_seed(0)
+    gn, x = nn.GroupNorm(2, 8).double(), torch.randn(2, 8, 5, 5, dtype=torch.float64)
+    with torch.no_grad():
+        gn.weight.normal_()
+        gn.bias.normal_()
+    assert torch.equal(getattr(modules, call)(x, gn), after(gn(x)))
+
+
+@pytest.mark.parametrize("make", [lambda: build_model({"type": "wresnet40_2", "norm": "group"}, 7),
+                                  lambda: build_model({"type": "efficientnet-b0", "norm": "group"}, 7)])
+def test_group_models_answer_in_fp64(make):
+    """What a model gives in 64 bits is what it gives in 32, to the roundings of some forty or eighty layers."""
+    torch.manual_seed(0)
+    model = make().eval()
+    x = torch.randn(2, 3, 32, 32)
+    with torch.no_grad():
+        low, full = model(x), model.double()(x.double())
+    assert full.dtype == torch.float64
+    assert (low - full).abs().max() <= 1e-4 * full.abs().max()
