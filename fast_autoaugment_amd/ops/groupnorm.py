@@ -79,9 +79,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
 class GroupNormAct(torch.nn.GroupNorm):
     """nn.GroupNorm on ``group_norm_act`` where that has x's type; ``ops.modules`` fuses the activation that follows it."""
 
-    act = "none"
-
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype not in DTYPES:
             return super().forward(x)
-        return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act)
+        return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps)

@@ -86,12 +86,10 @@ def conv1x1_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 class LinearAct(torch.nn.Linear):
     """nn.Linear on ``linear_act`` where x has the weights' type (under autocast it may not: torch's product then)."""
 
-    act = "none"
-
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype != self.weight.dtype or x.dtype not in DTYPES:
             return torch.nn.functional.linear(x, self.weight, self.bias)
-        return linear_act(x, self.weight, self.bias, act=self.act)
+        return linear_act(x, self.weight, self.bias)
 
 
 def fuse_pointwise(model: torch.nn.Module) -> int:
