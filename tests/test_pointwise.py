@@ -376,3 +376,66 @@ def test_a_gradient_that_is_no_number_stays_in_its_row_and_column(dev, act, t, m
     assert torch.equal(dx[rows], dx0[rows]) and torch.equal(dw[cols], dw0[cols]) and torch.equal(db[cols], db0[cols])
     dr[7, 5] = dr0[7, 5]
     assert torch.equal(dr, dr0)
+
+
+# forward tiles of 128x128, 128x64, 64x64, 32x32; dW's k split in 256, 2, 64, 42 and 17, or not; lines that are widened;
+# k of the forward product and of dx split; one chunk of rows, or many, for db
+WHOLE = [(70001, 64, 64), (3001, 392, 1000), (70001, 64, 256), (90001, 264, 136), (40003, 264, 136), (50003, 61, 35),
+         (20011, 16, 96), (131, 4000, 72), (33, 520, 5003), (131, 1152, 48), (9001, 128, 520), (130, 5, 2047)]
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("t", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,k,n", WHOLE)
+def test_sums_of_whole_numbers_are_exact(dev, act, t, m, k, n):
+    """Products and sums of small whole numbers are exact in fp32 in any order: results are theirs, rounded once, so
+    that a part of a sum that is lost or counted twice shows, however long the sum is."""
+    g = torch.Generator().manual_seed(m + k + n)
+    whole = lambda most, *s: torch.randint(-most, most + 1, s, generator=g).to(t)  # noqa: E731
+    x, w, b, r, dy = whole(2, m, k), whole(2, n, k), whole(3, n), whole(3, m, n), whole(2, m, n)
+    z = x.float() @ w.float().t() + b.float() + r.float()        # below 2^24 throughout
+    assert 4 * max(m, n, k) + 6 < 2 ** 24
+    dz = torch.where(z > 0, dy, torch.zeros_like(dy)) if act == "relu" else dy
+    leaves = [v.to(dev).requires_grad_(True) for v in (x, w, b, r)]
+    y = linear_act(leaves[0], leaves[1], leaves[2], leaves[3], act=act)
+    got = torch.autograd.grad(y, leaves, dy.to(dev))
+    want = [dz.float() @ w.float(), dz.float().t() @ x.float(), dz.double().sum(0), dz]
+    assert torch.equal(y.detach().cpu(), (z.relu() if act == "relu" else z).to(t))
+    for name, a, c in zip(("dx", "dw", "db", "dr"), got, want):
+        assert torch.equal(a.cpu(), c.to(t)), name
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act", ["swish", "sigmoid"])
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("m,k,n", WHOLE)
+def test_both_numbers_of_a_gradient_reach_every_part_of_a_sum(dev, act, t, m, k, n):
+    """x (or W) has two rows with 1 and -1 in each column, spread over the whole sum, and zeros: a column of dW (dx) is
+    the difference of two rows of dz, which are near each other, so that what bf16 or fp16 leaves of one would show.
+    Their slopes (see above) and the two numbers of each are off as before, and four terms are added."""
+    g = torch.Generator().manual_seed(m + k + n + 1)
+    r = lambda *s: torch.randn(*s, generator=g).to(t)  # noqa: E731
+    rows = m if m >= n else n                                   # the longer sum: dW's or dx's
+    at = torch.randperm(rows, generator=g)[:2 * k] if rows >= 2 * k else torch.randint(0, rows, (2 * k,), generator=g)
+    at[0], at[-1] = 0, rows - 1
+    pick = torch.zeros(rows, k, dtype=t)
+    first, second = at[:k], at[k:]
+    pick[first, torch.arange(k)], pick[second, torch.arange(k)] = 1.0, -1.0
+    x, w = (pick, r(n, k)) if rows == m else (r(m, k), pick)
+    b, res, dy = r(n), (r(m, 1) * 2.0 ** -6).expand(m, n).contiguous() + r(1, n), r(1, n).expand(m, n).contiguous()
+    if rows == n:
+        b, res, dy = r(n) * 2.0 ** -6, r(m, 1).expand(m, n).contiguous(), r(m, 1).expand(m, n).contiguous()
+    o = oracle(x, w, b, res, act, dy)
+    leaves = [v.to(dev).requires_grad_(True) for v in (x, w)]
+    y = linear_act(leaves[0], leaves[1], b.to(dev), residual=res.to(dev), act=act)
+    dx, dw = torch.autograd.grad(y, leaves, dy.to(dev))
+    u, f = torch.finfo(t).eps / 2, 2.0 ** -24
+    z_off = (k + 4) * f * o["size"] + 2 * f * o["z"].abs()
+    off = o["dy64"].abs() * (o["bend"] * z_off + 8 * f) + u * u * o["dz"].abs() + (2.0 ** -36 if t == FP16 else 2.0 ** -133)
+    dz, side = o["dz"].abs(), pick.double().abs()
+    if rows == m:
+        got, want, tol = dw, o["dw"], off.t() @ side + 8 * f * (dz.t() @ side)
+    else:
+        got, want, tol = dx, o["dx"], off @ side + 8 * f * (dz @ side)
+    close(got, want, u * (want.abs() + tol) + tol + torch.finfo(t).tiny * u)
