@@ -314,3 +314,97 @@ def test_offsets_beyond_32_bits(shape, groups):
     # one sample's sums may be cut in other parts there: a step of bf16, and of values near 0 one of those near 1
     for a, b in ((y[-2:], y2), (dx[-2:], dx2)):
         assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -12)
+
+
+def offset_bounds(x, groups, w, b, act, dy, chain=96, eps=1e-5):
+    """The gradients in 64 bits, and how far fp32 arithmetic may be off them where a mean lies far from zero.
+
+    f is half a step of fp32, `most` the largest |x| rstd of a group, and no sum is longer than `chain` additions in a
+    row. A mean is off by chain f of |x|, and so is each xhat, in spreads: `shift` = chain f most. z = x a + c adds four
+    roundings of that size. What follows is linear in `most`: sum dz xhat may be taken as rstd sum dz x + c sum dz, whose
+    terms are |dz| most, and dx as dz a + (x p + q), whose last terms are |mean u xhat| most."""
+    f = 2.0 ** -24
+    n, c = x.shape[:2]
+    s = oracle(x, groups, w, b, eps, act, dy)
+    col = (1, c) + (1,) * (x.dim() - 2)
+    w64, b64, dy64 = w.double().view(col), b.double().view(col), s["dy"].double()
+    per = lambda t: t.reshape(n, groups, -1)  # noqa: E731
+    back = lambda t: t.expand(n, groups, per(x).size(2)).reshape(x.shape)  # noqa: E731
+    mean = lambda t: back(per(t).mean(2, keepdim=True))  # noqa: E731
+    g = per(x.double())
+    d = g - g.mean(2, keepdim=True)
+    r = (d.square().mean(2, keepdim=True) + eps).rsqrt()
+    xhat, most, rs = back(d * r), back(g.abs().amax(2, keepdim=True) * r), back(r)
+    z = xhat * w64 + b64
+    sig = torch.sigmoid(z)
+    slope, bend = (sig * (1 + z * (1 - sig)), 0.5) if act == "swish" else (torch.ones_like(z), 0.0)
+    dz = dy64 * slope
+    u, shift = dz * w64, chain * f * most
+    m1, m2 = mean(u).abs(), mean(u * xhat).abs()
+    z_err = w64.abs() * (shift + 4 * f * most) + 2 * f * (z.abs() + b64.abs())
+    dz_err = (dy64.abs() * (bend * z_err + 8 * f) if act == "swish" else 0.0) + 2 * f * dz.abs()
+    u_err = dz_err * w64.abs() + f * u.abs()
+    m1_err = mean(u_err) + chain * f * mean(u.abs())
+    m2_err = mean(u_err * xhat.abs()) + (2 * chain * f * most + shift) * mean(u.abs())
+    # both factors of the last term are off: (xhat + d)(m2 + e) - xhat m2 = xhat e + d m2 + d e, with d up to
+    # shift + 6 f most, and the last of these is no smaller than the others where a large group's m2 is near 0
+    dx = rs * (u_err + m1_err + xhat.abs() * m2_err + (m2 + m2_err) * (shift + 6 * f * most)
+               + (chain + 8) * f * (u.abs() + m1 + xhat.abs() * m2))
+    red = [0] + list(range(2, x.dim()))
+    dw = (dz_err * xhat.abs() + (2 * chain * f * most + shift) * dz.abs() + (chain + 8) * f * (dz * xhat).abs()).sum(red)
+    db = (dz_err + chain * f * dz.abs()).sum(red)
+    return s, [(s["dx"], dx), (s["dw"], dw), (s["db"], db)]
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("shape,groups", [((2, 16, 40, 40), 8), ((2, 16, 150, 150), 8), ((2, 15, 20, 20), 5), ((3, 64, 28, 28), 16),
+                                          ((2, 256, 56, 56), 64), ((40, 24, 6, 6), 6), ((2, 12, 31, 33), 4), ((500, 16, 2, 2), 2)])
+def test_a_variance_between_channels_with_a_mean_far_from_zero(dev, shape, groups):
+    """Channels that lie a spread apart at a mean of 1000: the variance is that of their means, whose rounding at 1000
+    (6e-5) is no part of it. It is a sum of squares of at most 64 additions in a row, each 2^-24 of it, around a mean
+    that is off by at most 64 2^-24 of 1000 spreads, which the variance has squared; rstd has half of these, and the
+    quotient and root three roundings. rstd is what the results say: the regression of y - mean y on x - mean x, where
+    errors that all values share fall out and those of their own, 2 2^-24 of up to 4 each, are averaged."""
+    g = torch.Generator().manual_seed(9)
+    n, c = shape[:2]
+    x = 1000.0 + torch.randn(1, c, 1, 1, generator=g) + 0.05 * torch.randn(*shape, generator=g)
+    y = group_norm_act(x.to(dev), groups).cpu().double().reshape(n, groups, -1)
+    d = x.double().reshape(n, groups, -1)
+    d = d - d.mean(2, keepdim=True)
+    var = d.square().mean(2)
+    want = (var + 1e-5).rsqrt()
+    got = (d * (y - y.mean(2, keepdim=True))).mean(2) / var
+    f, most = 2.0 ** -24, 1010.0 * want
+    assert ((got / want - 1).abs() <= 32 * f + 0.5 * (64 * f * most) ** 2 + 3 * f + 8 * f).all()
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("act,mean", [("none", 1000.0), ("none", 30.0), ("swish", 30.0), ("swish", -30.0), ("swish", 3.0)])
+@pytest.mark.parametrize("shape,groups", [((2, 16, 40, 40), 2), ((2, 16, 150, 150), 2), ((2, 15, 20, 20), 3),
+                                          ((3, 64, 28, 28), 8), ((2, 256, 56, 56), 32), ((40, 24, 6, 6), 4)])
+def test_gradients_with_a_mean_far_from_zero(dev, act, mean, shape, groups):
+    """The digits that the mean costs its own rounding are all that it costs a gradient."""
+    x, w, b, dy = inputs(shape, FP32, mean=mean)
+    s, bounds = offset_bounds(x, groups, w, b, act, dy)
+    for want, tol in bounds:        # what is no gradient does not pass
+        for wrong in (torch.zeros_like(want), -want):
+            assert ((wrong - want).abs() > tol + 2.0 ** -24 * want.abs()).any()
+    leaves = [t.to(dev).requires_grad_(True) for t in (x, w, b)]
+    y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act)
+    got = torch.autograd.grad(y, leaves, s["dy"].to(dev))
+    for name, a, (want, tol) in zip(("dx", "dw", "db"), got, bounds):
+        err, tol = (a.cpu().double() - want).abs(), tol + 2.0 ** -24 * want.abs()
+        assert (err <= tol).all(), f"{name} off by {float((err / tol).max()):.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("t", [FP32, BF16])
+@pytest.mark.parametrize("where", [(0, 0, 0), (-1, -1, -1), (1, 3, 2)])
+@pytest.mark.parametrize("shape,groups", [((2, 16, 40, 40), 2), ((2, 16, 150, 150), 2), ((2, 15, 20, 20), 3), ((3, 64, 1, 2), 8)])
+def test_an_outlier_wherever_it_lies(dev, t, where, shape, groups):
+    """One value ten thousand times the others, at a group's ends or within: it costs the others no digits."""
+    x, w, b, dy = inputs(shape, t)
+    c, h, v = (i % n if i < 0 else min(i, n - 1) for i, n in zip(where, (shape[1] // groups, *shape[2:])))
+    x[:, c, h, v] = 1e4
+    x[:, shape[1] // groups + c, h, v] = -1e4
+    check(dev, x, groups, w, b, "none", dy)
