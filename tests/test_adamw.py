@@ -580,3 +580,26 @@ def test_a_state_of_other_weights_is_refused():
     with pytest.raises(ValueError):
         opt.load_state_dict({**sd, "exp_avg": torch.zeros_like(before), "flat_master": torch.zeros(3)})
     assert torch.equal(opt.exp_avg, before)
+
+
+@pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [0.0, 1.0])
+def test_flat_fp16_follows_the_formula(dev, bits, clip):
+    model, flat = flat_model(dev, torch.float16)
+    opt = FusedAdamW(flat, lr=1e-2, weight_decay=0.1, grad_clip=clip, state_bits=bits)
+    places = [((p.data_ptr() - flat.flat_param.data_ptr()) // p.element_size(), p.numel()) for p in flat.params]
+    weights = [flat.flat_master[o:o + n] for o, n in places]
+    for step in range(3):
+        g = torch.Generator().manual_seed(step)
+        for p in flat.params:
+            p.grad.copy_(torch.randn(p.shape, generator=g))
+        before = state_of(opt, weights, places)
+        opt.step()
+        check_step(opt, before, [flat.flat_grad[o:o + n] for o, n in places], weights,
+                   [0.1 if o < flat.n_decay else 0.0 for o, _ in places], 1e-2, clip)
+        assert torch.equal(flat.flat_param, flat.flat_master.half())
+    used = torch.zeros(flat.numel, dtype=torch.bool)
+    for o, n in places:
+        used[o:o + n] = True
+    assert not flat.flat_master.cpu()[~used].any() and not flat.flat_param.cpu()[~used].any()

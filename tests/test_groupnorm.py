@@ -398,6 +398,22 @@ def test_gradients_with_a_mean_far_from_zero(dev, act, mean, shape, groups):
 
 
 @pytest.mark.parametrize("dev", DEV)
+@pytest.mark.parametrize("t", [FP32, BF16, FP16])
+@pytest.mark.parametrize("shape,groups", [((2, 4096, 3, 3), 1), ((3, 8192, 2, 2), 2), ((1, 16384, 2, 1), 1), ((2, 32768, 3, 1), 2),
+                                          ((2, 6001, 5, 5), 1), ((1, 2049, 1, 1), 1), ((70, 4104), 2), ((1, 16384, 30, 30), 1)])
+def test_groups_of_many_channels(dev, t, shape, groups):
+    """More channels a group than a workgroup holds: up to 16384, whose sums wait in LDS until they are joined."""
+    x, w, b, dy = inputs(shape, t)
+    check(dev, x, groups, w, b, "swish", dy)
+
+
+@GPU
+def test_a_group_of_too_many_channels_is_refused():
+    with pytest.raises(RuntimeError, match="16384"):
+        group_norm_act(torch.zeros(2, 16385, device="cuda"), 1)
+
+
+@pytest.mark.parametrize("dev", DEV)
 @pytest.mark.parametrize("t", [FP32, BF16])
 @pytest.mark.parametrize("where", [(0, 0, 0), (-1, -1, -1), (1, 3, 2)])
 @pytest.mark.parametrize("shape,groups", [((2, 16, 40, 40), 2), ((2, 16, 150, 150), 2), ((2, 15, 20, 20), 3), ((3, 64, 1, 2), 8)])
