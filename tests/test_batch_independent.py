@@ -330,3 +330,34 @@ def test_group_models_answer_in_fp64(make):
         low, full = model(x), model.double()(x.double())
     assert full.dtype == torch.float64
     assert (low - full).abs().max() <= 1e-4 * full.abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_from_the_same_gradients_are_the_cpu_s(dtype, bits):
+    """Both devices are given the CPU's gradients of a batch: weights then differ by an update's own roundings (about 32
+    of it, below 2 lr in size here) and by those of the weight and its decay, step by step."""
+    flats, opts, lr = [], [], 1e-3
+    for dev in ("cpu", "cuda"):
+        torch.manual_seed(0)
+        model = build_model({"type": "wresnet40_2", "norm": "group"}, 7).to(dev)
+        flats.append(flatten_module(model, align=256, work_dtype=dtype))
+        opts.append(FusedAdamW(flats[-1], lr=lr, weight_decay=0.05, state_bits=bits))
+    torch.manual_seed(0)
+    source = build_model({"type": "wresnet40_2", "norm": "group"}, 7)
+    grads = flatten_module(source, align=256)
+    g = torch.Generator().manual_seed(1)
+    weights = lambda f: (f.flat_param if f.flat_master is None else f.flat_master).cpu()  # noqa: E731
+    for done in range(1, 4):
+        nn.functional.cross_entropy(source(torch.randn(4, 3, 32, 32, generator=g)), torch.arange(4)).backward()
+        for f, opt in zip(flats, opts):
+            before = weights(f).clone()
+            f.flat_grad.copy_(grads.flat_grad)
+            opt.step()
+        a, b = (weights(f) for f in flats)
+        assert ((a - b).abs() <= done * (4 * 2.0 ** -24 * a.abs() + 2 * lr * 32 * 2.0 ** -24)).all()
+        assert (a - before).abs().max() > lr / 2
+        for name in opts[0]._names:
+            x, y = (getattr(o, name).cpu() for o in opts)
+            assert torch.equal(x.float(), y.float()), name
