@@ -21,6 +21,7 @@ tensors, one more for the step's scalars and one for the norm if it clips.
 from __future__ import annotations
 
 import math
+import operator
 import struct
 
 import torch
@@ -346,6 +347,7 @@ class FusedAdamW:
         self._dev = f.flat_param.device
         self._items = [(0, nd, self.weight_decay), (nd, n - nd, 0.0)]
         self._flat_stamp = None
+        self._counted = [p for p in f.params if not p.is_inference()]
         return n
 
     def _init_list(self, params):
@@ -392,7 +394,7 @@ class FusedAdamW:
         if f.flat_param.dtype == torch.float32:
             return
         # a parameter of the buffer counts its own writes
-        stamp = (*self._stamp(f.flat_param), sum(self._stamp(p)[1] for p in f.params))
+        stamp = (*self._stamp(f.flat_param), sum(map(operator.attrgetter("_version"), self._counted)))
         if stamp == self._flat_stamp:
             return
         if self._dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
