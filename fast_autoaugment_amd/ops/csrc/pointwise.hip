@@ -31,6 +31,12 @@
 // what reads the result next pays for them: 25088x1024x256 and a product back
 // 53 for 47.
 // Products of a few hundred rows take 3 to 6 us, which is a launch.
+//
+// Swish and sigmoid keep their slope in fp32 for the backward pass, and dz enters
+// its products as two numbers of 16 bits, at twice the steps of k and twice the
+// reads of dz: the gradients of 128x1152x48 in bf16 are then off by the rounding
+// of the results alone (0.0019 of their norm, 0.0024 with a dz of 16 bits), and its
+// two products take 4.1 + 4.5 us for 3.4 + 3.5.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>

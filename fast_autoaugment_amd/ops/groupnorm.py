@@ -68,7 +68,9 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     ``weight`` and ``bias`` are [C] or None, in x's type or fp32. ``act`` is
     "none", "relu" or "swish". Everything is computed in fp32 and rounded once.
     On the GPU the result is channels last (a map of another order is copied
-    into it first), and gradients go to x, weight and bias, once.
+    into it first), and gradients go to x, weight and bias, once. There a sample
+    has fewer than 2^31 values, a group at most 16384 channels, and N times the
+    groups, or the workgroups they are cut into, stay below 2^24; more is refused.
     """
     _check(x, num_groups, weight, bias, eps, act)
     if not x.is_cuda:

@@ -45,6 +45,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     for swish and sigmoid the slopes are kept for them in fp32, and for 16-bit
     types the backward products take the gradient behind the activation as a sum
     of two numbers of that type, which holds 16 (bf16) or 22 (fp16) bits of it.
+    On the GPU x has fewer than 2^31 - 256 rows, K and N are 2^23 at most, and a
+    result has fewer than 2^24 tiles; more is refused.
     """
     _check(x, weight, bias, residual, act)
     C = require_ext_for(x)

@@ -361,3 +361,38 @@ def test_steps_from_the_same_gradients_are_the_cpu_s(dtype, bits):
         for name in opts[0]._names:
             x, y = (getattr(o, name).cpu() for o in opts)
             assert torch.equal(x.float(), y.float()), name
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """Calls that run beside each other have workspaces of their own: chunks, joins, split and small products."""
+    from fast_autoaugment_amd.ops.groupnorm import group_norm_act
+    from fast_autoaugment_amd.ops.pointwise import linear_act
+    g = torch.Generator("cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()  # noqa: E731
+
+    def norm(x, w, b, dy):
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        y = group_norm_act(x, 4, w, b, act="swish")
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    def product(x, w, b, dy):
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        y = linear_act(x, w, b, act="swish")
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    cases = [(norm, [r(4, 16, 130, 130), r(16), r(16), r(4, 16, 130, 130)]), (norm, [r(9, 64, 14, 14), r(64), r(64), r(9, 64, 14, 14)]),
+             (product, [r(20000, 64), r(96, 64), r(96), r(20000, 96)]), (product, [r(131, 4000), r(72, 4000), r(72), r(131, 72)]),
+             (product, [r(3001, 61), r(35, 61), r(35), r(3001, 35)])]
+    alone = [f(*args) for f, args in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(20):
+        torch.cuda.synchronize()
+        out = []
+        for s, k in zip(streams, (i % 5, (i // 5 + i + 1) % 5)):
+            with torch.cuda.stream(s):
+                out.append((k, cases[k][0](*cases[k][1])))
+        torch.cuda.synchronize()
+        for k, got in out:
+            for a, b in zip(got, alone[k]):
+                assert torch.equal(a, b)
