@@ -15,11 +15,14 @@
 // the pass before read is still in the last-level cache. The same in slices of
 // samples that would stay there whole was slower: 136 + 237 us in two of them.
 //
-// Statistics are sums around the mean in fp32, never a difference of squares. Means
-// are taken of x - base, where base is a value of the group (the middle one of three,
-// which no single outlier is): parts of a group are joined by their means, whose
-// rounding would else cost the variance the digits that a mean far from zero has
-// (rstd 3e-5 off at a mean of 1000 spreads). It costs 0.2 us of 10.
+// Statistics are sums around the mean in fp32, never a difference of squares.
+// Parts of a group are joined by their means, whose rounding costs the variance the
+// digits that a mean far from zero has (rstd up to 1e-4 off at a mean of 1000
+// spreads). That is no more than a 16-bit map's own rounding; means of fp32 maps are
+// taken of x - base, where base is a value of the group (the middle one of three,
+// which no single outlier is). It costs them up to 5 % of the forward pass
+// (128x28x28x512 91 us for 87); 16-bit maps it would cost 36 us for 29 at
+// 128x56x56x64, where one round of workgroups is bound by instructions.
 // Sums over pixels are taken channel by channel, in a fixed order: a thread owns
 // VEC neighbouring channels, the rows of threads are added through LDS, and
 // channels are joined to groups last, so a group may be any number of channels.
@@ -263,14 +266,32 @@ __device__ __forceinline__ void read_vec(const float* table, int c, float (&out)
   for (int j = 0; j < VEC; ++j) out[j] = table[c + j];
 }
 
-// A value of channel c's group in a sample x, the same for all parts of the group: the middle one of its first, a central
-// and its last. Where one of them is no number, so is the group.
-template <typename T>
-__device__ __forceinline__ float group_base(const T* x, int c, int S, int C, int cg) {
+// whether a map's values are taken less a value near their mean
+template <typename T> constexpr bool kCentred = sizeof(T) == 4;
+
+// A value of the group of each of VEC channels from c in a sample x, the same for all parts of the group: the middle one
+// of its first, a central and its last. Where one of them is no number, so is the group. A wave has one x.
+template <typename T, int VEC>
+__device__ __forceinline__ void group_base(const T* x, int c, int S, int C, int cg, float (&base)[VEC]) {
   typedef Pack<T, 1> P;
-  const int first = c / cg * cg;
-  auto at = [&](int p, int ch) { return P::get(*(const typename P::raw*)(x + (int64_t)p * C + first + ch), 0); };
-  return __builtin_amdgcn_fmed3f(at(0, 0), at(S / 2, cg / 2), at(S - 1, cg - 1));
+  const T *central = x + (int64_t)(S / 2) * C + cg / 2, *last = x + (int64_t)(S - 1) * C + cg - 1;
+  auto of = [&](int first) {
+    const uint32_t off = (uint32_t)first * sizeof(T);
+    return __builtin_amdgcn_fmed3f(P::get(load_at<T, 1>(x, off), 0), P::get(load_at<T, 1>(central, off), 0),
+                                   P::get(load_at<T, 1>(last, off), 0));
+  };
+  int first = c / cg * cg;
+  if (cg >= VEC) {            // one group, or two where a vector is no part of it
+    const float one = of(first), two = cg % VEC == 0 ? one : of((c + VEC - 1) / cg * cg);
+    #pragma unroll
+    for (int j = 0; j < VEC; ++j) base[j] = c + j - first < cg ? one : two;
+    return;
+  }
+  #pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    if (c + j - first >= cg) first += cg;
+    base[j] = of(first);
+  }
 }
 
 // mean (less base) and sum of squares around it of a thread's own pixels, channel by channel
@@ -286,17 +307,26 @@ __device__ __forceinline__ void own_moments(const Tile& t, const typename Pack<T
     if (t.on && t.r + i * t.rows < np) {
       n += 1.0f;
       #pragma unroll
-      for (int j = 0; j < VEC; ++j) mean[j] += P::get(raw[i], j) - base[j];
+      for (int j = 0; j < VEC; ++j) {
+        float v = P::get(raw[i], j);
+        if constexpr (kCentred<T>) v -= base[j];
+        mean[j] += v;
+      }
     }
   const float inv = n > 0.0f ? 1.0f / n : 0.0f;
+  float around[VEC];        // base is no part of the squares: what rounds here they have squared
   #pragma unroll
-  for (int j = 0; j < VEC; ++j) mean[j] *= inv;
+  for (int j = 0; j < VEC; ++j) {
+    mean[j] *= inv;
+    around[j] = mean[j];
+    if constexpr (kCentred<T>) around[j] += base[j];
+  }
   #pragma unroll
   for (int i = 0; i < R; ++i)
     if (t.on && t.r + i * t.rows < np) {
       #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float d = P::get(raw[i], j) - base[j] - mean[j];
+        const float d = P::get(raw[i], j) - around[j];
         m2[j] += d * d;
       }
     }
@@ -332,17 +362,14 @@ __global__ __launch_bounds__(256) void gn_chunk_stats_kernel(
   const T* xb = x + (b * S + p0) * C + c0;
   const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
   typedef Pack<T, VEC> P;
-  float* out = lds + 2 * blockDim.x * VEC + 8;      // the channels' bases first
-  float one = (int)threadIdx.x < t.ch ? group_base<T>(x + b * S * C, c0 + threadIdx.x, S, C, cg) : 0.0f;
   typename P::raw raw[R];
   #pragma unroll
   for (int i = 0; i < R; ++i)
     if (t.on && t.r + i * t.rows < np) raw[i] = load_at<T, VEC>(xb, off + i * step);
-  if ((int)threadIdx.x < t.ch) out[threadIdx.x] = one;      // a tile is 256 channels at most
-  __syncthreads();
   float base[VEC], mean[VEC], m2[VEC];
-  read_vec<VEC>(out, t.v * VEC, base);
+  if constexpr (kCentred<T>) group_base<T, VEC>(x + b * S * C, c0 + t.v * VEC, S, C, cg, base);
   own_moments<T, VEC, R>(t, raw, np, base, mean, m2);
+  float* out = lds + 2 * blockDim.x * VEC + 8;
   channel_moments<VEC>(t, mean, m2, np, lds, out);
   float* to = ws + (b * nchunk + ck) * 2 * C + c0;
   for (int c = threadIdx.x; c < t.ch; c += blockDim.x) {
@@ -419,7 +446,8 @@ __global__ __launch_bounds__(256) void gn_join_stats_kernel(
   const int lane = threadIdx.x & 63;
   for (int g = (int)threadIdx.x >> 6; g < j.groups; g += 4) {
     float s = 0.0f, q = 0.0f;
-    const float base = group_base<T>(x + j.b * S * C, (j.g0 + g) * cg, S, C, cg);
+    float base[1] = {0.0f};
+    if constexpr (kCentred<T>) group_base<T, 1>(x + j.b * S * C, (j.g0 + g) * cg, S, C, cg, base);
     for (int c = lane; c < cg; c += 64) s += lds[g * cg + c];
     const float mean = wave_sum(s) / (float)cg;
     for (int c = lane; c < cg; c += 64) {
@@ -428,7 +456,7 @@ __global__ __launch_bounds__(256) void gn_join_stats_kernel(
     }
     const float rstd = 1.0f / sqrtf(wave_sum(q) / ((float)cg * (float)S) + eps);
     if (lane == 0) {
-      mean_out[j.b * G + j.g0 + g] = base + mean;
+      mean_out[j.b * G + j.g0 + g] = base[0] + mean;
       rstd_out[j.b * G + j.g0 + g] = rstd;
     }
   }
@@ -438,8 +466,10 @@ __global__ __launch_bounds__(256) void gn_join_stats_kernel(
 
 // z = x a + c with a = rstd w, c = b - mean a;  xhat = x rstd + shift with shift = -mean rstd;
 // dx = dz a + x p + q with p = -rstd^2 m2, q = -rstd m1 - shift rstd m2   (m1, m2: means of u, u xhat).
-// A mean far from zero costs these the digits that it costs the mean itself; so it does to
-// sum dz xhat = rstd sum dz x + shift sum dz, which leaves the loop with two constants a channel.
+// A mean far from zero costs y the digits that it costs the mean itself. It would cost sum dz xhat = rstd sum dz x +
+// shift sum dz more: at a mean of 30 spreads, dw 3e-6 of itself where the formula loses 7e-7. That is far below what
+// 16-bit maps hold, whose loops have these two constants a channel; for fp32 maps the backward pass subtracts the mean
+// first: with x - mean in the place of x, c is b, shift 0 and q = -rstd m1 (128x28x28x512 160 us for 153).
 // A workgroup makes them once for its tile, in LDS; a thread then has those of its VEC channels.
 template <typename T, int VEC, int R>
 __global__ __launch_bounds__(256) void gn_chunk_apply_kernel(
@@ -489,7 +519,7 @@ __global__ __launch_bounds__(256) void gn_chunk_apply_kernel(
   });
 }
 
-// the constants of the backward pass's first half: {rstd, shift, a, c} x tile
+// the constants of the backward pass's first half: {rstd, shift or mean, a, c} x tile
 template <typename T>
 __device__ __forceinline__ void backward_table(float* table, int tile, int ch, int c0, int cg,
                                                const float* mean, const float* rstd, const void* w,
@@ -498,9 +528,9 @@ __device__ __forceinline__ void backward_table(float* table, int tile, int ch, i
     const int g = (c0 + c) / cg;
     const float r = rstd[g], shift = -mean[g] * r, wc = param<T>(w, f32, c0 + c, 1.0f);
     table[c] = r;
-    table[tile + c] = shift;
+    table[tile + c] = kCentred<T> ? mean[g] : shift;
     table[2 * tile + c] = r * wc;
-    table[3 * tile + c] = param<T>(bias, f32, c0 + c, 0.0f) + shift * wc;
+    table[3 * tile + c] = param<T>(bias, f32, c0 + c, 0.0f) + (kCentred<T> ? 0.0f : shift * wc);
   }
 }
 
@@ -529,6 +559,8 @@ __global__ __launch_bounds__(256) void gn_chunk_grads_kernel(
   #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[0][j] = acc[1][j] = 0.0f;
   if (t.on) {
+    float mu[VEC];        // of fp32 maps
+    if constexpr (kCentred<T>) read_vec<VEC>(table + tile, t.v * VEC, mu);
     float a[VEC], c[VEC];
     read_vec<VEC>(table + 2 * tile, t.v * VEC, a);
     read_vec<VEC>(table + 3 * tile, t.v * VEC, c);
@@ -547,7 +579,8 @@ __global__ __launch_bounds__(256) void gn_chunk_grads_kernel(
           if (t.r + (o + i) * t.rows < np) {
             #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-              const float xv = P::get(xr[i], j);
+              float xv = P::get(xr[i], j);
+              if constexpr (kCentred<T>) xv -= mu[j];
               const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
               acc[0][j] += dz;
               acc[1][j] += dz * xv;
@@ -560,7 +593,7 @@ __global__ __launch_bounds__(256) void gn_chunk_grads_kernel(
   float* out = ws + (b * nchunk + ck) * 2 * C + c0;
   for (int i = threadIdx.x; i < t.ch; i += blockDim.x) {
     out[i] = sums[i];
-    out[C + i] = table[i] * sums[t.ch + i] + table[tile + i] * sums[i];
+    out[C + i] = table[i] * sums[t.ch + i] + (kCentred<T> ? 0.0f : table[tile + i] * sums[i]);
   }
 }
 
@@ -627,7 +660,7 @@ __global__ __launch_bounds__(256) void gn_chunk_dx_kernel(
     const void* __restrict__ bias, bool f32, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ means, T* __restrict__ dx, int S, int C,
     int cg, int tile, int ntile, int nchunk, int chunk, int act) {
-  extern __shared__ float lds[];                // {a, c, p, q} x tile
+  extern __shared__ float lds[];                // {a, c, p, q, mean} x tile
   // last chunks first: they were read last, and may still be in the cache behind the L2s
   const uint32_t wg = gridDim.x - 1 - blockIdx.x, at_tile = wg / (uint32_t)ntile, at_chunk = at_tile / (uint32_t)nchunk;
   const int ti = (int)(wg - at_tile * ntile), ck = (int)(at_tile - at_chunk * nchunk);
@@ -643,12 +676,15 @@ __global__ __launch_bounds__(256) void gn_chunk_dx_kernel(
     const float r = rstd[g], shift = -mean[g] * r, wc = param<T>(w, f32, c0 + c, 1.0f);
     const float m1 = means[2 * g], m2 = means[2 * g + 1];
     lds[c] = r * wc;
-    lds[tile + c] = param<T>(bias, f32, c0 + c, 0.0f) + shift * wc;
+    lds[tile + c] = param<T>(bias, f32, c0 + c, 0.0f) + (kCentred<T> ? 0.0f : shift * wc);
     lds[2 * tile + c] = -r * r * m2;
-    lds[3 * tile + c] = -r * (m1 + shift * m2);
+    lds[3 * tile + c] = -r * (m1 + (kCentred<T> ? 0.0f : shift * m2));
+    if (kCentred<T>) lds[4 * tile + c] = mean[g];
   }
   __syncthreads();
   if (!t.on) return;
+  float mu[VEC];        // of fp32 maps
+  if constexpr (kCentred<T>) read_vec<VEC>(lds + 4 * tile, t.v * VEC, mu);
   float a[VEC], c[VEC], pp[VEC], q[VEC];
   read_vec<VEC>(lds, t.v * VEC, a);
   read_vec<VEC>(lds + tile, t.v * VEC, c);
@@ -670,7 +706,8 @@ __global__ __launch_bounds__(256) void gn_chunk_dx_kernel(
           typename P::raw out;
           #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const float xv = P::get(xr[i], j);
+            float xv = P::get(xr[i], j);
+            if constexpr (kCentred<T>) xv -= mu[j];
             const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
             P::set(out, j, dz * a[j] + (xv * pp[j] + q[j]));
           }
@@ -709,20 +746,20 @@ __global__ __launch_bounds__(1024) void gn_whole_fwd_kernel(
   const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
   float* channels = lds + 2 * blockDim.x * VEC + 8; // {mean, m2} x channels
   float* groups = channels + 2 * tile;              // {mean, rstd} x groups
-  float* bases = groups + 2 * tile;                 // channels
+  float* bases = groups + 2 * tile;                 // channels, of fp32 maps
   typedef Pack<T, VEC> P;
-  const T* sample = x + b * S * C;
-  float one = (int)threadIdx.x < t.ch ? group_base<T>(sample, c0 + threadIdx.x, S, C, cg) : 0.0f;
   typename P::raw raw[R];
   #pragma unroll
   for (int i = 0; i < R; ++i)
     if (t.on && t.r + i * t.rows < S) raw[i] = load_at<T, VEC>(x + at, off + i * step);
-  if ((int)threadIdx.x < t.ch) bases[threadIdx.x] = one;
-  for (int c = threadIdx.x + blockDim.x; c < t.ch; c += blockDim.x) bases[c] = group_base<T>(sample, c0 + c, S, C, cg);
-  __syncthreads();
   float base[VEC], m[VEC], m2[VEC];
-  read_vec<VEC>(bases, t.v * VEC, base);
+  if constexpr (kCentred<T>) group_base<T, VEC>(x + b * S * C, c0 + t.v * VEC, S, C, cg, base);
   own_moments<T, VEC, R>(t, raw, S, base, m, m2);
+  if constexpr (kCentred<T>)
+    if (t.r == 0) {
+      #pragma unroll
+      for (int j = 0; j < VEC; ++j) bases[t.v * VEC + j] = base[j];
+    }
   channel_moments<VEC>(t, m, m2, S, lds, channels);
   const int64_t g0 = b * (C / cg) + c0 / cg;
   const int lane = threadIdx.x & 63;
@@ -736,7 +773,7 @@ __global__ __launch_bounds__(1024) void gn_whole_fwd_kernel(
     }
     const float rstd = 1.0f / sqrtf(wave_sum(q) / ((float)cg * (float)S) + eps);
     if (lane == 0) {
-      groups[2 * g] = mean_out[g0 + g] = bases[g * cg] + mean;
+      groups[2 * g] = mean_out[g0 + g] = kCentred<T> ? bases[g * cg] + mean : mean;
       groups[2 * g + 1] = rstd;
       rstd_out[g0 + g] = rstd;
     }
@@ -783,7 +820,7 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
   const Tile t(min(tile, C - c0), VEC);
   const int64_t at = b * S * C + c0, g0 = b * (C / cg);
   const uint32_t off = (uint32_t)(t.r * C + t.v * VEC) * sizeof(T), step = (uint32_t)(t.rows * C) * sizeof(T);
-  float* table = lds + 2 * blockDim.x * VEC;    // {rstd, shift, a, c} x tile
+  float* table = lds + 2 * blockDim.x * VEC;    // {rstd, shift or mean, a, c} x tile
   float* sums = table + 4 * tile;               // {dz, dz xhat} x channels
   float* groups = sums + 2 * tile;              // {u, u xhat} x groups
   typedef Pack<T, VEC> P;
@@ -798,6 +835,8 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
   }
   backward_table<T>(table, tile, t.ch, c0, cg, mean_in + g0, rstd_in + g0, w, bias, f32);
   __syncthreads();
+  float mu[VEC];        // of fp32 maps
+  if constexpr (kCentred<T>) read_vec<VEC>(table + tile, t.v * VEC, mu);
   float a[VEC], c[VEC];
   read_vec<VEC>(table + 2 * tile, t.v * VEC, a);
   read_vec<VEC>(table + 3 * tile, t.v * VEC, c);
@@ -810,7 +849,8 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
       if (t.on && t.r + i * t.rows < S) {
         #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float xv = P::get(xr[i], j);
+          float xv = P::get(xr[i], j);
+          if constexpr (kCentred<T>) xv -= mu[j];
           const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
           acc[0][j] += dz;
           acc[1][j] += dz * xv;
@@ -819,7 +859,7 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
   });
   channel_sums<VEC, 2>(t, acc, lds, sums);
   for (int i = threadIdx.x; i < t.ch; i += blockDim.x) {
-    const float s1 = sums[i], s2 = table[i] * sums[t.ch + i] + table[tile + i] * s1;
+    const float s1 = sums[i], s2 = table[i] * sums[t.ch + i] + (kCentred<T> ? 0.0f : table[tile + i] * s1);
     const float wc = param<T>(w, f32, c0 + i, 1.0f);
     sample[b * 2 * C + c0 + i] = s1;
     sample[(b * 2 + 1) * C + c0 + i] = s2;
@@ -831,7 +871,8 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
   const float inv = 1.0f / ((float)cg * (float)S);
   for (int i = threadIdx.x; i < t.ch; i += blockDim.x) {
     const int g = i / cg;
-    const float m1 = groups[g] * inv, m2 = groups[t.ch / cg + g] * inv, r = table[i], shift = table[tile + i];
+    const float m1 = groups[g] * inv, m2 = groups[t.ch / cg + g] * inv, r = table[i],
+                shift = kCentred<T> ? 0.0f : table[tile + i];
     table[i] = -r * r * m2;
     table[tile + i] = -r * (m1 + shift * m2);
   }
@@ -848,7 +889,8 @@ __global__ __launch_bounds__(1024) void gn_whole_bwd_kernel(
         typename P::raw out;
         #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float xv = P::get(xr[i], j);
+          float xv = P::get(xr[i], j);
+          if constexpr (kCentred<T>) xv -= mu[j];
           const float dz = act_grad<A.value>(P::get(dr[i], j), xv * a[j] + c[j]);
           P::set(out, j, dz * a[j] + (xv * pp[j] + q[j]));
         }
@@ -1045,7 +1087,7 @@ void forward_on(const Shape& s, const torch::Tensor& x, const void* w, const voi
              hipStream_t stream) {
   Whole p;
   if (whole_of<T, VEC, kForwardR<T, VEC>>(s, p)) {
-    const size_t lds = (2 * (size_t)p.threads * VEC + 8 + 5 * p.tile) * sizeof(float);
+    const size_t lds = (2 * (size_t)p.threads * VEC + 8 + (kCentred<T> ? 5 : 4) * p.tile) * sizeof(float);
     auto go = [&](auto kern) {
       hipLaunchKernelGGL(kern, dim3((unsigned)(s.B * p.ntile)), dim3(p.threads), lds, stream,
                          (const T*)x.data_ptr(), w, b, f32, (T*)y.data_ptr(), mean.data_ptr<float>(),
@@ -1101,7 +1143,7 @@ torch::Tensor backward_on(const Shape& s, const torch::Tensor& dy, const torch::
                      (2 * gt * s.cg + 512) * sizeof(float), stream, ws.data_ptr<float>(), w, f32,
                      means.data_ptr<float>(), sample.data_ptr<float>(), s.S, s.C, s.cg, gt, c.nchunk);
   hipLaunchKernelGGL((gn_chunk_dx_kernel<T, VEC, kR, 4>), dim3((unsigned)c.wgs), dim3(256),
-                     4 * c.tile * sizeof(float), stream,
+                     (kCentred<T> ? 5 : 4) * c.tile * sizeof(float), stream,
                      (const T*)dy.data_ptr(), (const T*)x.data_ptr(), w, b, f32,
                      mean.data_ptr<float>(), rstd.data_ptr<float>(), means.data_ptr<float>(),
                      (T*)dx.data_ptr(), s.S, s.C, s.cg, c.tile, c.ntile, c.nchunk, c.chunk, act);

@@ -424,3 +424,24 @@ def test_an_outlier_wherever_it_lies(dev, t, where, shape, groups):
     x[:, c, h, v] = 1e4
     x[:, shape[1] // groups + c, h, v] = -1e4
     check(dev, x, groups, w, b, "none", dy)
+
+
+@GPU
+@pytest.mark.parametrize("mean", [1000.0, 30.0, 0.5])
+@pytest.mark.parametrize("act", ["none", "swish"])
+@pytest.mark.parametrize("shape,groups", [((2, 16, 150, 150), 2), ((2, 16, 40, 40), 2), ((2, 256, 56, 56), 32), ((2, 15, 20, 20), 3)])
+def test_results_lose_no_more_than_the_formula_in_fp32(mean, act, shape, groups):
+    """The kernels' errors against 64 bits, as a share of a result's norm, are at most twice those of the formula that
+    torch computes step by step in fp32, where x less its mean comes first, and four roundings: both are off by what the
+    mean's rounding costs (which may be more on one side than on the other) and by their sums' own."""
+    from fast_autoaugment_amd.ops.groupnorm import _composed
+    x, w, b, dy = inputs(shape, FP32, mean=mean)
+    want = oracle(x, groups, w, b, 1e-5, act, dy)
+    off = []
+    for fn in (lambda *v: group_norm_act(v[0], groups, v[1], v[2], act=act), lambda *v: _composed(v[0], groups, v[1], v[2], 1e-5, act)):
+        leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+        y = fn(*leaves)
+        got = [y.detach(), *torch.autograd.grad(y, leaves, dy.cuda())]
+        off.append([float((a.cpu().double() - want[k]).norm() / want[k].norm()) for a, k in zip(got, ("y", "dx", "dw", "db"))])
+    for k, ours, formula in zip(("y", "dx", "dw", "db"), *off):
+        assert ours <= 2 * formula + 4 * 2.0 ** -24, (k, ours, formula)
