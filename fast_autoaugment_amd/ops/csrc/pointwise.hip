@@ -33,10 +33,11 @@
 // Products of a few hundred rows take 3 to 6 us, which is a launch.
 //
 // Swish and sigmoid keep their slope in fp32 for the backward pass, and dz enters
-// its products as two numbers of 16 bits, at twice the steps of k and twice the
-// reads of dz: the gradients of 128x1152x48 in bf16 are then off by the rounding
-// of the results alone (0.0019 of their norm, 0.0024 with a dz of 16 bits), and its
-// two products take 4.1 + 4.5 us for 3.4 + 3.5.
+// its products as two numbers of 16 bits: the gradients of 128x1152x48 in bf16 are
+// then off by the rounding of the results alone (0.0019 of their norm, 0.0024 with a
+// sum and a dz of 16 bits). That is 10 bytes more a value of the result to write and
+// read, in all passes: 128x1152x48 trained takes 80 us for 78, where a launch counts,
+// 25088x1024x256 126 for 92 and 100352x128x512 340 for 213, where memory does.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -300,13 +301,13 @@ struct Loader {
       if (row0 + row >= o.rows) off[i] = 0xffffffffu;
     }
   }
-  // The pieces of k0 .. k0+63 to lds. Reads behind the operand's end give zeros; so do k that are not there, and
+  // The pieces of k0 .. k0+63 to lds, of the operand or of one `second` bytes further. Reads behind the operand's end give zeros; so do k that are not there, and
   // all of a step that is not wanted: none of these touches memory.
-  __device__ __forceinline__ void operator()(int k0, bool wanted, short* lds, int wave) const {
+  __device__ __forceinline__ void operator()(int k0, bool wanted, short* lds, int wave, int64_t second = 0) const {
     const int64_t skip = ROWS ? k0 * line : (int64_t)k0 * 2;
     const int64_t rest = wanted ? left - skip : 0;
     const uint32_t bytes = rest > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)rest;
-    auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + skip), 0, bytes, 0x00020000);
+    auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(base + skip + second), 0, bytes, 0x00020000);
     typedef __attribute__((address_space(3))) void* lds_t;
     #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -326,7 +327,8 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t wg, uint32_t n) {
 // ------------------------------------------------------------ the product in 16 bits
 
 // Operands with contiguous rows are those of the gradients, which have no bias, residual or activation.
-// TWO: P has two terms. What is left over goes first, then the sums are scaled back and the rounded values follow.
+// TWO: P has two terms. Every step is taken twice, with what is left over (even) and with the rounded values (odd): the
+// second finds its piece of Q in the L2. A pass for each took 131 us for 126 at 25088x1024x256 trained.
 template <typename T, bool PR, bool QR, int BM, int BN, bool TWO>
 __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, Epilogue<T> epi,
                                                       float* __restrict__ part, int tiles_m,
@@ -341,29 +343,38 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
   const int tn = (int)(id - id_m * tiles_n), tm = (int)(id_m - sp * tiles_m);
   const int m0 = tm * BM, n0 = tn * BN;
   const int steps = (P.kdim + BK - 1) / BK;
-  const int s0 = (int)((int64_t)steps * sp / splits), s1 = (int)((int64_t)steps * (sp + 1) / splits);
+  const int s0 = (int)((int64_t)steps * sp / splits) * (TWO ? 2 : 1),
+            s1 = (int)((int64_t)steps * (sp + 1) / splits) * (TWO ? 2 : 1);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (wave >> 1) * (BM / 2), wn = (wave & 1) * (BN / 2);
   const int M = P.rows, N = Q.rows;
-  LP load_p(P, m0, tid);
+  const LP load_p(P, m0, tid);
   const LQ load_q(Q, n0, tid);
 
-  f32x4 acc[FM][FN];
+  f32x4 acc[FM][FN], left[TWO ? FM : 1][TWO ? FN : 1];
   #pragma unroll
   for (int i = 0; i < FM; ++i)
     #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int j = 0; j < FN; ++j) {
+      acc[i][j] = f32x4{0, 0, 0, 0};
+      if constexpr (TWO) left[i][j] = acc[i][j];
+    }
 
   auto fill = [&](int s, short* p, short* q) {
-    load_p(s * BK, s < s1, p, wave);
-    load_q(s * BK, s < s1, q, wave);
+    if constexpr (TWO) {
+      load_p(s / 2 * BK, s < s1, p, wave, s % 2 == 0 ? P.second : 0);
+      load_q(s / 2 * BK, s < s1, q, wave);
+    } else {
+      load_p(s * BK, s < s1, p, wave);
+      load_q(s * BK, s < s1, q, wave);
+    }
   };
   // The older of two steps' pieces have come, here and in the other waves. Loads end in order and every step
   // asks for as many, so a count says so; other loads in flight only make it stricter.
   auto come = [] { asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(LP::N + LQ::N) : "memory"); };
   // all waves have read their fragments: the buffer may be filled again
   auto read = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-  auto multiply = [&](const short* p, const short* q) {
+  auto add = [&](const short* p, const short* q, auto& acc) {
     #pragma unroll
     for (int k = 0; k < BK; k += 32) {
       s16x8 fp[FM], fq[FN];
@@ -376,6 +387,12 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
         #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
     }
+  };
+  auto multiply = [&](const short* p, const short* q) { add(p, q, acc); };
+  // the first buffers have even steps; in bf16, where nothing is scaled, both kinds share their sums
+  auto multiply_even = [&](const short* p, const short* q) {
+    if constexpr (TWO && Num<T>::kSecond != 1.0f) add(p, q, left);
+    else add(p, q, acc);
   };
   const int mine = n0 + wn + (lane >> 4) * 8;       // the lane's first column
   // the residual is on its way during the product; where there is none to read at once, zeros are read from nowhere
@@ -393,38 +410,31 @@ __global__ __launch_bounds__(256, 2) void product_kernel(Operand P, Operand Q, E
         res[i][j / 2] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, mine + j * 16 < N ? at : 0xffffffffu, 0, 0);
       }
   }
-  auto steps_of_k = [&] {
-    fill(s0, p0, q0);
-    fill(s0 + 1, p1, q1);
-    int s = s0;
-    for (; s + 2 < s1; s += 2) {
-      come();
-      multiply(p0, q0);
-      read();
-      fill(s + 2, p0, q0);
-      come();
-      multiply(p1, q1);
-      read();
-      fill(s + 3, p1, q1);
-    }
-    if (s < s1) {     // one or two steps are left; no others are asked for
-      come();
-      multiply(p0, q0);
-    }
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 1 < s1) multiply(p1, q1);
-  };
-  if constexpr (TWO) {
-    load_p.base += P.second;
-    steps_of_k();
-    load_p.base -= P.second;
+  fill(s0, p0, q0);
+  fill(s0 + 1, p1, q1);
+  int s = s0;
+  for (; s + 2 < s1; s += 2) {
+    come();
+    multiply_even(p0, q0);
+    read();
+    fill(s + 2, p0, q0);
+    come();
+    multiply(p1, q1);
+    read();
+    fill(s + 3, p1, q1);
+  }
+  if (s < s1) {     // one or two steps are left; no others are asked for
+    come();
+    multiply_even(p0, q0);
+  }
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  if (s + 1 < s1) multiply(p1, q1);
+  if constexpr (TWO && Num<T>::kSecond != 1.0f) {
     #pragma unroll
     for (int i = 0; i < FM; ++i)
       #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] *= 1.0f / Num<T>::kSecond;
-    read();           // the buffers are filled again
+      for (int j = 0; j < FN; ++j) acc[i][j] += left[i][j] * (1.0f / Num<T>::kSecond);
   }
-  steps_of_k();
 
   // lane: output row lane%16 of a fragment; of fragments j, j+1 columns (lane/16)*8 + 0..3 and + 4..7
   auto each = [&](auto f) {
@@ -478,16 +488,21 @@ __global__ __launch_bounds__(256) void small_product_kernel(Operand P, Operand Q
   __shared__ __align__(16) short p0[4][B * BK], p1[4][B * BK], q0[4][B * BK], q1[4][B * BK];
   const uint32_t tm = blockIdx.x / (uint32_t)tiles_n;
   const int m0 = (int)tm * B, n0 = (int)(blockIdx.x - tm * tiles_n) * B;
-  const int steps = (P.kdim + BK - 1) / BK;
+  const int steps = (P.kdim + BK - 1) / BK * (TWO ? 2 : 1);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  LP load_p(P, m0, lane);
+  const LP load_p(P, m0, lane);
   const LQ load_q(Q, n0, lane);
   f32x4 acc[2][2];
   #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = f32x4{0, 0, 0, 0};
   auto fill = [&](int s, short* p, short* q) {
-    load_p(s * BK, s < steps, p, 0);
-    load_q(s * BK, s < steps, q, 0);
+    if constexpr (TWO) {      // see product_kernel: waves 0 and 2 have what is left over, 1 and 3 the rounded values
+      load_p(s / 2 * BK, s < steps, p, 0, s % 2 == 0 ? P.second : 0);
+      load_q(s / 2 * BK, s < steps, q, 0);
+    } else {
+      load_p(s * BK, s < steps, p, 0);
+      load_q(s * BK, s < steps, q, 0);
+    }
   };
   // the older of two steps' pieces have come (see product_kernel); fragments are read, and may be overwritten
   auto come = [] { asm volatile("s_waitcnt vmcnt(%0)" ::"i"(LP::N + LQ::N) : "memory"); };
@@ -507,29 +522,24 @@ __global__ __launch_bounds__(256) void small_product_kernel(Operand P, Operand Q
         for (int j = 0; j < 2; ++j) acc[i][j] = Num<T>::mfma(fq[j], fp[i], acc[i][j]);
     }
   };
-  auto steps_of_k = [&] {
-    fill(wave, p0[wave], q0[wave]);
-    fill(wave + 4, p1[wave], q1[wave]);
-    for (int s = wave; s < steps; s += 8) {
-      come();
-      multiply(p0[wave], q0[wave]);
-      read();
-      fill(s + 8, p0[wave], q0[wave]);
-      come();
-      multiply(p1[wave], q1[wave]);       // zeros where the step is not there
-      read();
-      fill(s + 12, p1[wave], q1[wave]);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  };
-  if constexpr (TWO) {      // see product_kernel
-    load_p.base += P.second;
-    steps_of_k();
-    load_p.base -= P.second;
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] *= 1.0f / Num<T>::kSecond;
+  fill(wave, p0[wave], q0[wave]);
+  fill(wave + 4, p1[wave], q1[wave]);
+  for (int s = wave; s < steps; s += 8) {
+    come();
+    multiply(p0[wave], q0[wave]);
+    read();
+    fill(s + 8, p0[wave], q0[wave]);
+    come();
+    multiply(p1[wave], q1[wave]);       // zeros where the step is not there
+    read();
+    fill(s + 12, p1[wave], q1[wave]);
   }
-  steps_of_k();
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if constexpr (TWO) {
+    const float scale = wave % 2 == 0 ? 1.0f / Num<T>::kSecond : 1.0f;
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] *= scale;
+  }
   __syncthreads();
   // the waves' sums, 32 lines of 32 and 4 more (a line's start moves by 4 banks)
   constexpr int LD = B + 4;
