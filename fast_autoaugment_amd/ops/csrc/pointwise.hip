@@ -143,12 +143,12 @@ __device__ __forceinline__ float act_value(float z) {
   if (ACT == ACT_SIGMOID) return sigmoid(z);
   return z;
 }
+// activations whose slope is kept for the backward pass
+template <int ACT> constexpr bool kept = ACT == ACT_SWISH || ACT == ACT_SIGMOID;
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   const float s = sigmoid(z);
-  if (ACT == ACT_SWISH) return s + s * (z - z * s);
-  if (ACT == ACT_SIGMOID) return s - s * s;
-  return 1.0f;
+  return ACT == ACT_SWISH ? s + s * (z - z * s) : s - s * s;
 }
 // f(activation as a constant): one branch outside the loops, not one an element
 template <bool ANY = true, typename F>
@@ -190,12 +190,13 @@ struct Epilogue {
     const int64_t at = m * N + n;
     if (bias) v += load4(bias + n, left, vec);
     if (res) v += load4(res + at, left, vec);
-    if (slope) {
-      f32x4 d;
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = act_slope<ACT>(v[i]);
-      store4(slope + at, left, vec, d);
-    }
+    if constexpr (kept<ACT>)
+      if (slope) {
+        f32x4 d;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = act_slope<ACT>(v[i]);
+        store4(slope + at, left, vec, d);
+      }
     #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = act_value<ACT>(v[i]);
     store4(y + at, left, vec, v);
@@ -203,13 +204,14 @@ struct Epilogue {
   // 8 columns, 16 bytes at once; bias and residual are in v
   template <int ACT>
   __device__ __forceinline__ void eight(int64_t at, f32x8 v) const {
-    if (slope) {
-      f32x4 d[2];
-      #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e >> 2][e & 3] = act_slope<ACT>(v[e]);
-      *(f32x4*)(slope + at) = d[0];
-      *(f32x4*)(slope + at + 4) = d[1];
-    }
+    if constexpr (kept<ACT>)
+      if (slope) {
+        f32x4 d[2];
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) d[e >> 2][e & 3] = act_slope<ACT>(v[e]);
+        *(f32x4*)(slope + at) = d[0];
+        *(f32x4*)(slope + at + 4) = d[1];
+      }
     s16x8 out;
     #pragma unroll
     for (int e = 0; e < 8; ++e) out[e] = Num<T>::bits(act_value<ACT>(v[e]));
